@@ -1,4 +1,5 @@
 """Loaders of the shared libraries: libnq_hybrid.so (kernels of hybrid decoders, include/nq_hybrid_ops.h, ctypes),
+libnq_mx.so (microscaled formats, include/nq_mx_ops.h) with its operators in libnq_mx_torch.so,
 libawq_hip.so (the C ABI declared in include/awq_hip.h and
 include/nq_engine_ops.h, bound with ctypes) and libawq_torch.so (the PyTorch operator binding over that ABI for the
 linear path: torch.ops.nanoquantization_amd.*).
@@ -168,6 +169,19 @@ HYBRID_SYMBOLS = {
     "nqh_decode_advance": (_int, [_vp] * 6 + [_i64] * 2 + [_vp]),
 }
 
+# symbol -> (restype, argtypes) of libnq_mx.so; every symbol of include/nq_mx_ops.h
+MX_SYMBOLS = {
+    "nqx_last_error": (ctypes.c_char_p, []),
+    "nqx_quantize": (_int, [_vp, _i64, _vp, _vp, _i64, _i64, _int, _int, _vp]),
+    "nqx_dequantize": (_int, [_vp, _vp, _vp, _i64, _i64, _int, _int, _vp]),
+    "nqx_linear_quantized": (_int, [_vp] * 6 + [_i64] * 3 + [_int, _int, _vp]),
+    "nqx_linear_workspace_bytes": (_sz, [_i64] * 3 + [_int, _int]),
+    "nqx_linear": (_int, [_vp, _i64] + [_vp] * 4 + [_i64] * 3 + [_int, _int, _vp, _sz, _vp]),
+    "nqx_linear_form": (ctypes.c_char_p, [_i64] * 3 + [_int] * 3),
+    "nqx_add_rmsnorm": (_int, [_vp, _i64, _vp, _i64] + [_vp] * 4 + [_i64, _i64, _f32, _int, _int, _vp]),
+    "nqx_silu_mul": (_int, [_vp, _i64, _vp, _i64, _vp, _vp, _i64, _i64, _int, _int, _vp]),
+}
+
 
 class AwqHipError(RuntimeError):
     pass
@@ -217,6 +231,54 @@ def check_hybrid(status: int) -> None:
     if status != 0:
         msg = hybrid_lib().nqh_last_error().decode("utf-8", "replace")
         raise AwqHipError(f"libnq_hybrid: {_STATUS.get(status, status)}: {msg}")
+
+
+MX_LIB_PATH = os.path.join(PKG_DIR, "libnq_mx.so")
+MX_TORCH_LIB_PATH = os.path.join(PKG_DIR, "libnq_mx_torch.so")
+_mx = None
+_mx_ops = None
+
+
+def mx_lib() -> ctypes.CDLL:
+    """The kernels of microscaled formats (include/nq_mx_ops.h); raises if they have not been built."""
+    global _mx
+    if _mx is None:
+        with _lock:
+            if _mx is None:
+                if not os.path.exists(MX_LIB_PATH):
+                    raise AwqHipError(
+                        f"{MX_LIB_PATH} is missing: build it with `python -m nanoquantization_amd.build` "
+                        "(there is no CPU or eager fallback for the MX kernels)")
+                handle = ctypes.CDLL(MX_LIB_PATH)
+                for name, (res, args) in MX_SYMBOLS.items():
+                    fn = getattr(handle, name)
+                    fn.restype, fn.argtypes = res, args
+                _mx = handle
+    return _mx
+
+
+def check_mx(status: int) -> None:
+    if status != 0:
+        msg = mx_lib().nqx_last_error().decode("utf-8", "replace")
+        raise AwqHipError(f"libnq_mx: {_STATUS.get(status, status)}: {msg}")
+
+
+def mx_ops():
+    """torch.ops.nanoquantization_amd with the operators of csrc/mx/mx_binding.cpp (mx_quantize, mx_dequantize, mx_linear,
+    mx_linear_quantized, mx_add_rmsnorm, mx_rmsnorm, mx_silu_mul), registered by loading libnq_mx_torch.so.  Raises if it has
+    not been built."""
+    global _mx_ops
+    if _mx_ops is None:
+        mx_lib()                                        # first: the binding links against it
+        with _lock:
+            if _mx_ops is None:
+                if not os.path.exists(MX_TORCH_LIB_PATH):
+                    raise AwqHipError(
+                        f"{MX_TORCH_LIB_PATH} is missing: build it with `python -m nanoquantization_amd.build` "
+                        "(there is no CPU or eager fallback for the MX kernels)")
+                torch.ops.load_library(MX_TORCH_LIB_PATH)
+                _mx_ops = torch.ops.nanoquantization_amd
+    return _mx_ops
 
 
 TORCH_LIB_PATH = os.path.join(PKG_DIR, "libawq_torch.so")

@@ -1,5 +1,6 @@
-"""Builds csrc/*.hip into nanoquantization_amd/libawq_hip.so for gfx950, csrc/hybrid/*.hip into libnq_hybrid.so, and csrc/torch_binding.cpp (host code
-only: the PyTorch operator registration over the C ABI) into nanoquantization_amd/libawq_torch.so.
+"""Builds csrc/*.hip into nanoquantization_amd/libawq_hip.so for gfx950, csrc/hybrid/*.hip into libnq_hybrid.so, csrc/mx/*.hip into libnq_mx.so, and
+csrc/torch_binding.cpp and csrc/mx/mx_binding.cpp (host code only: the PyTorch operator registration over the C ABIs) into
+nanoquantization_amd/libawq_torch.so and libnq_mx_torch.so.
 
 Usage: python -m nanoquantization_amd.build
 """
@@ -17,7 +18,11 @@ LIB_PATH = os.path.join(PKG_DIR, "libawq_hip.so")
 HYBRID_CSRC = os.path.join(CSRC, "hybrid")
 HYBRID_LIB_PATH = os.path.join(PKG_DIR, "libnq_hybrid.so")
 
+MX_CSRC = os.path.join(CSRC, "mx")
+MX_LIB_PATH = os.path.join(PKG_DIR, "libnq_mx.so")
+
 TORCH_LIB_PATH = os.path.join(PKG_DIR, "libawq_torch.so")
+MX_TORCH_LIB_PATH = os.path.join(PKG_DIR, "libnq_mx_torch.so")
 
 ROCM = os.environ.get("ROCM_PATH", "/opt/rocm")
 HIPCC = os.environ.get("HIPCC", os.path.join(ROCM, "bin", "hipcc"))
@@ -63,22 +68,36 @@ def _run(cmd, verbose):
         print(out)
 
 
-def build_hybrid(verbose: bool = True) -> str:
-    """Compile csrc/hybrid/*.hip (in parallel) and link libnq_hybrid.so: all that the hybrid decoders need."""
+def _build_folder(csrc: str, name: str, lib: str, verbose: bool) -> str:
+    """Compile csrc/*.hip (in parallel) and link them into `lib`."""
     from concurrent.futures import ThreadPoolExecutor
 
-    objdir = os.path.join(PKG_DIR, "build", "hybrid")
+    objdir = os.path.join(PKG_DIR, "build", name)
     os.makedirs(objdir, exist_ok=True)
     compile_flags = [f for f in FLAGS if f != "-shared"]
-    srcs = sorted(glob.glob(os.path.join(HYBRID_CSRC, "*.hip")))
+    srcs = sorted(glob.glob(os.path.join(csrc, "*.hip")))
     objs = [os.path.join(objdir, os.path.basename(s) + ".o") for s in srcs]
     with ThreadPoolExecutor(max_workers=8) as pool:
         list(pool.map(lambda so: _run([HIPCC, *compile_flags, *EXTRA.get(os.path.basename(so[0]), []), "-c", so[0],
                                        "-o", so[1]], verbose), zip(srcs, objs)))
-    part = f"{HYBRID_LIB_PATH}.{os.getpid()}"       # a second process never sees half a library
+    part = f"{lib}.{os.getpid()}"       # a second process never sees half a library
     _run([HIPCC, "--offload-arch=gfx950", "-shared", "-fPIC", *objs, "-o", part], verbose)
-    os.replace(part, HYBRID_LIB_PATH)
-    return HYBRID_LIB_PATH
+    os.replace(part, lib)
+    return lib
+
+
+def build_hybrid(verbose: bool = True) -> str:
+    """Compile csrc/hybrid/*.hip (in parallel) and link libnq_hybrid.so: all that the hybrid decoders need."""
+    return _build_folder(HYBRID_CSRC, "hybrid", HYBRID_LIB_PATH, verbose)
+
+
+def build_mx(verbose: bool = True) -> str:
+    """libnq_mx.so from csrc/mx/*.hip, and its operators, libnq_mx_torch.so: all that the microscaled formats need."""
+    _build_folder(MX_CSRC, "mx", MX_LIB_PATH, verbose)
+    obj = os.path.join(PKG_DIR, "build", "mx", "mx_binding.o")
+    _run(torch_binding_compile_cmd(obj, os.path.join(MX_CSRC, "mx_binding.cpp")), verbose)
+    _run(torch_binding_link_cmd(obj, MX_TORCH_LIB_PATH, "nq_mx"), verbose)
+    return MX_LIB_PATH
 
 
 def ensure_hybrid() -> None:
@@ -92,6 +111,7 @@ def build(verbose: bool = True) -> str:
     from concurrent.futures import ThreadPoolExecutor
 
     build_hybrid(verbose)
+    build_mx(verbose)
     objdir = os.path.join(PKG_DIR, "build")
     os.makedirs(objdir, exist_ok=True)
     compile_flags = [f for f in FLAGS if f != "-shared"]
@@ -117,17 +137,17 @@ def _torch_dirs():
             os.path.join(root, "lib"), int(torch._C._GLIBCXX_USE_CXX11_ABI))
 
 
-def torch_binding_compile_cmd(obj: str) -> list[str]:
+def torch_binding_compile_cmd(obj: str, source: str = os.path.join(CSRC, "torch_binding.cpp")) -> list[str]:
     incs, _, abi = _torch_dirs()
     return [CXX, "-O2", "-fPIC", "-std=c++17", "-w", "-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM=1",
             f"-D_GLIBCXX_USE_CXX11_ABI={abi}", *[f"-I{i}" for i in incs], f"-I{ROCM}/include",
-            "-c", os.path.join(CSRC, "torch_binding.cpp"), "-o", obj]
+            "-c", source, "-o", obj]
 
 
-def torch_binding_link_cmd(obj: str) -> list[str]:
+def torch_binding_link_cmd(obj: str, lib: str = TORCH_LIB_PATH, over: str = "awq_hip") -> list[str]:
     _, libdir, _ = _torch_dirs()
-    return [CXX, "-shared", "-fPIC", obj, "-o", TORCH_LIB_PATH, f"-L{libdir}", "-ltorch", "-ltorch_cpu", "-lc10",
-            "-lc10_hip", "-ltorch_hip", f"-L{PKG_DIR}", "-lawq_hip", "-ldl", "-Wl,-rpath,$ORIGIN", f"-Wl,-rpath,{libdir}"]
+    return [CXX, "-shared", "-fPIC", obj, "-o", lib, f"-L{libdir}", "-ltorch", "-ltorch_cpu", "-lc10",
+            "-lc10_hip", "-ltorch_hip", f"-L{PKG_DIR}", f"-l{over}", "-ldl", "-Wl,-rpath,$ORIGIN", f"-Wl,-rpath,{libdir}"]
 
 
 if __name__ == "__main__":

@@ -1,0 +1,52 @@
+// Launchers of the products of libnq_mx.so; mx_linear.hip chooses among them.
+#pragma once
+
+#include "mx_common.hpp"
+
+namespace nqx {
+
+// y [rows, n] = x . w^T + bias; w [n, k / 2] e2m1 and ws [n, k / 32].
+struct Product {
+    const uint8_t* x;
+    const uint8_t* xs;
+    const uint8_t* w;
+    const uint8_t* ws;
+    const void* bias;
+    void* y;
+    int64_t rows, n, k;
+    int dtype, format;
+};
+
+// One matrix instruction: 16 weight rows x 16 rows of x over 128 values (four blocks).  Lane l has row l % 16 and, with
+// g = l / 16, block g in e2m1 (16 bytes); in e4m3 the 16 bytes of values 16 g .. and those of 64 + 16 g ...  Its scale byte
+// is that of block g for either type.  The result: column l % 16, weight rows 4 g .. 4 g + 3.
+template <int FORMAT>
+__device__ __forceinline__ f32x4 mfma(u32x4 w, u32x4 x0, u32x4 x1, f32x4 c, uint32_t w_scale, uint32_t x_scale) {
+    const i32x8 a = {(int)w[0], (int)w[1], (int)w[2], (int)w[3], 0, 0, 0, 0};
+    const i32x8 b = {(int)x0[0], (int)x0[1], (int)x0[2], (int)x0[3], (int)x1[0], (int)x1[1], (int)x1[2], (int)x1[3]};
+    return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, b, c, 4, FORMAT == NQX_FP4 ? 4 : 0, 0, (int)w_scale, 0, (int)x_scale);
+}
+
+// Four consecutive values of a row of y, columns n .. n + 3 of which those below N exist.
+template <typename T>
+__device__ __forceinline__ void store_sums(f32x4 v, typename T::elem* y, const typename T::elem* bias, int64_t row, int64_t n,
+                                           int64_t N) {
+    typename T::elem* to = y + row * N + n;
+    if (bias) {
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+            if (n + r < N) v[r] += T::to_f32(bias[n + r]);
+    }
+    if ((N & 3) == 0) {          // then n + 3 < N, and the four are aligned
+        if constexpr (sizeof(typename T::elem) == 4) *reinterpret_cast<f32x4*>(to) = v;
+        else *reinterpret_cast<u32x2*>(to) = u32x2{T::pack2(v[0], v[1]), T::pack2(v[2], v[3])};
+    } else {
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+            if (n + r < N) to[r] = T::from_f32(v[r]);
+    }
+}
+
+int skinny_product(const Product& p, hipStream_t stream);
+
+}  // namespace nqx

@@ -1,0 +1,487 @@
+"""Microscaled operators on the GPU against their definition in 64 bits (oracle/mx_oracle.py)."""
+import pytest
+import torch
+
+import nanoquantization_amd as nq
+from nanoquantization_amd import _lib
+from oracle import mx_oracle as mx
+
+pytestmark = pytest.mark.gpu
+
+DT = {"f16": torch.float16, "bf16": torch.bfloat16, "f32": torch.float32}
+FORMATS = ("mxfp4", "mxfp8")
+U = 2.0 ** -24                                     # half a step of fp32, relative
+
+
+@pytest.fixture(autouse=True)
+def say(request):
+    print(request.node.name, flush=True)           # names the case before the GPU has it
+
+
+def _gen(seed):
+    return torch.Generator(device="cuda").manual_seed(seed)
+
+
+def _random(seed, *shape, dtype=torch.bfloat16, spread=True):
+    g = _gen(seed)
+    x = torch.randn(*shape, device="cuda", generator=g)
+    if spread:
+        x = x * torch.exp(torch.randn(shape[-1], device="cuda", generator=g))
+    return x.to(dtype)
+
+
+def _weight(seed, n, k):
+    return nq.mx_quantize(_random(seed, n, k, dtype=torch.float32, spread=False) * k ** -0.5, "mxfp4")
+
+
+def _equal_packed(got, want):
+    assert torch.equal(got[1].cpu(), want[1]), "scales"
+    assert torch.equal(got[0].cpu(), want[0]), "codes"
+
+
+# ---- quantise, dequantise: the definition's own codes ---------------------------------------------------------------------
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("dt", DT)
+@pytest.mark.parametrize("shape", [(1, 32), (3, 96), (2, 5, 160), (257, 2560), (7, 32 * 333), (64,)])
+def test_quantize_is_the_definition(shape, dt, fmt):
+    x = _random(len(shape) + shape[-1], *shape, dtype=DT[dt])
+    _equal_packed(nq.mx_quantize(x, fmt), mx.quantize(x, fmt))
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("dt", DT)
+def test_quantize_at_the_edges(dt, fmt):
+    """Ties, every magnitude of the type, zeros of both signs, the smallest and largest values, infinities and NaN."""
+    t = DT[dt]
+    top = torch.finfo(t).max
+    rows = []
+    for largest in (6.0, 7.0, 6.99, 4.0, 448.0, 464.0, 464.25, 480.0, 1.0, 2.0 ** -14):
+        r = torch.linspace(-1, 1, 32, dtype=torch.float64) * largest
+        rows.append(r)
+        rows.append(r.flip(0) * 0.25)
+    ties = torch.tensor([0.25, 0.75, 1.25, 1.75, 2.5, 3.5, 5.0, 6.0], dtype=torch.float64)
+    rows.append(torch.cat([ties, -ties, ties / 2, -ties / 4]))
+    e8 = mx.elements("mxfp8")
+    mid = (e8[1:] + e8[:-1]) / 2
+    rows += [torch.cat([mid[i:i + 31], e8[-1:]]) for i in range(0, 124, 31)]
+    rows += [torch.zeros(32, dtype=torch.float64), -torch.zeros(32, dtype=torch.float64)]
+    tiny = torch.finfo(t).smallest_normal * torch.finfo(t).eps             # the smallest subnormal
+    rows += [torch.full((32,), tiny, dtype=torch.float64), torch.arange(32, dtype=torch.float64) * tiny,
+             torch.full((32,), top, dtype=torch.float64), torch.linspace(-top, top, 32, dtype=torch.float64)]
+    for bad in (float("inf"), float("-inf"), float("nan")):
+        r = torch.linspace(-2, 2, 32, dtype=torch.float64)
+        r[13] = bad
+        rows.append(r)
+    x = torch.stack(rows).to(t)
+    got = nq.mx_quantize(x.cuda(), fmt)
+    _equal_packed(got, mx.quantize(x, fmt))
+    back = nq.mx_dequantize(*got, torch.float32).cpu()
+    assert torch.isnan(back[-3:]).all() and not torch.isnan(back[:-3]).any()
+    # the type's largest value may round up to 2^128, which fp32 has as infinity
+    assert torch.equal(back[:-3], mx.values(*got)[:-3].float())
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+def test_quantize_every_16_bit_value(fmt):
+    bits = torch.arange(1 << 16, dtype=torch.int32).to(torch.int16)
+    for t in (torch.bfloat16, torch.float16):
+        x = bits.view(t)
+        x = x[torch.isfinite(x)]
+        x = x[: x.numel() // 32 * 32].reshape(32, -1).t().contiguous()     # a block spans the range
+        _equal_packed(nq.mx_quantize(x.cuda(), fmt), mx.quantize(x, fmt))
+        flat = x.reshape(-1, 32)
+        near = flat.sort(0)[0].reshape(-1, 32)                            # and a block of neighbours
+        _equal_packed(nq.mx_quantize(near.cuda(), fmt), mx.quantize(near, fmt))
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("dt", DT)
+def test_dequantize_every_code_and_scale(dt, fmt):
+    """All codes under all scales; the value, exact in fp32, is rounded once."""
+    if fmt == "mxfp4":
+        codes = (torch.arange(256 * 16) % 256).to(torch.uint8).reshape(256, 16)
+        codes[:, 1::2] = codes[:, 1::2].flip(0)
+    else:
+        codes = torch.arange(256 * 32).remainder(256).to(torch.uint8).reshape(256, 32)
+    codes = codes.repeat(256, 1)
+    scales = torch.arange(256).repeat_interleave(256).to(torch.uint8).reshape(-1, 1)
+    got = nq.mx_dequantize(codes.cuda(), scales.cuda(), DT[dt]).cpu()
+    want = mx.values(codes, scales).float().to(DT[dt])
+    assert torch.equal(torch.isnan(got), torch.isnan(want))
+    assert torch.equal(got.nan_to_num(7.0, 1e4, -1e4), want.nan_to_num(7.0, 1e4, -1e4))
+    assert torch.equal(torch.signbit(got[~torch.isnan(got)]), torch.signbit(want[~torch.isnan(want)]))
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+def test_quantize_views(fmt):
+    """Rows of a wider tensor, a transposed one, one that starts off a 16-byte boundary, the same row many times, a row of rows."""
+    wide = _random(5, 37, 1024)
+    views = [wide[:, 128:128 + 320], wide[::2, 8:8 + 64], wide[:, 3:3 + 96], wide.t()[:, :32], wide[:1].expand(9, 1024),
+             wide[4], wide.view(37, 4, 256)[:, 1:3], wide[:, :64].unsqueeze(0), wide[1:2, 5:37]]
+    for v in views:
+        _equal_packed(nq.mx_quantize(v, fmt), mx.quantize(v, fmt))
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+def test_nothing_to_do(fmt):
+    x = torch.empty(0, 64, dtype=torch.bfloat16, device="cuda")
+    codes, scales = nq.mx_quantize(x, fmt)
+    assert codes.shape[0] == scales.shape[0] == 0 and nq.mx_dequantize(codes, scales).shape == (0, 64)
+    w, ws = _weight(1, 40, 64)
+    assert nq.mx_linear(x, w, ws, activations=fmt).shape == (0, 40)
+    assert nq.mx_linear(x.view(2, 0, 64), w, ws, activations=fmt).shape == (2, 0, 40)
+    assert nq.mx_linear_quantized(codes, scales, w, ws).shape == (0, 40)
+    assert nq.mx_linear(_random(1, 3, 64), w[:0], ws[:0], activations=fmt).shape == (3, 0)
+    assert nq.mx_add_rmsnorm(x, x, _random(1, 64), 1e-6, fmt)[2].shape == (0, 64)
+    assert nq.mx_silu_mul(x, x, fmt)[0].shape[0] == 0
+
+
+# ---- the product ----------------------------------------------------------------------------------------------------------
+def _exponents(codes, scales):
+    """The exponent that an element's code has, a zero's or subnormal's being the smallest, and the scale's."""
+    four = codes.shape[-1] == 16 * scales.shape[-1]
+    v = mx.values(codes, torch.full_like(scales, 127)).cuda()
+    e = (torch.frexp(torch.where(v == 0, 2.0 ** -20, v))[1] - 1).clamp_min(0 if four else -6)
+    return (e.unflatten(-1, (-1, 32)) + (scales.cuda().to(torch.int32) - 127).unsqueeze(-1)).flatten(-2)
+
+
+def _cut_off(x, ex, w, ew):
+    """What the matrix instruction loses of e4m3 products: it adds eight consecutive ones in fixed point, in units of 2^-13 of
+    the largest power of two that the exponents of a pair of codes give, and cuts off what is below (measured: 256 + 2^-5 is
+    exact and 256 + 2^-6 is 256 within an eight; from eight to eight the sum is one of fp32).  Products have six bits, so only
+    those below 2^-8 of that power lose any.  e2m1 products span fewer bits than that."""
+    (rows, k), n = x.shape, w.shape[0]
+    lost, step = [], max(1, 40_000_000 // (n * k))
+    for part, e in zip(x.abs().split(step), ex.split(step)):
+        p = (part.unsqueeze(1) * w.abs()).unflatten(-1, (-1, 8))
+        top = (e.unsqueeze(1) + ew).unflatten(-1, (-1, 8)).amax(-1, keepdim=True)
+        lost.append(p.remainder_(torch.ldexp(torch.ones_like(p[..., :1]), top - 13)).sum((-1, -2)))
+    return torch.cat(lost)
+
+
+def _check_product(y, x, weight, bias, dtype):
+    """|y - exact|: a value of y is a sum of k products, exact in fp32, by fp32 additions of which a product passes at most 128
+    within a matrix instruction, one more for every 128 values of k, eight where the waves' sums meet and the bias: each is off
+    by U of a partial sum, itself at most the sum of magnitudes.  e4m3 products lose what _cut_off says.  Then one rounding to
+    dtype, half a step of y or of the type's smallest value."""
+    x64, w64 = mx.values(*x).cuda(), mx.values(*weight).cuda()
+    k = x64.shape[-1]
+    want = torch.matmul(x64, w64.t())
+    size = torch.matmul(x64.abs(), w64.abs().t())
+    lost = _cut_off(x64, _exponents(*x), w64, _exponents(*weight)) if x[0].shape[-1] == k else 0.0
+    if bias is not None:
+        want, size = want + bias.double(), size + bias.double().abs()
+    info = torch.finfo(dtype)
+    tol = size * U * (128 + k / 128 + 9) * 1.01 + lost + (want.abs() + lost) * info.eps / 2 * 1.01 + info.smallest_normal * info.eps / 2
+    off = (y.double() - want).abs()
+    assert y.dtype == dtype and y.shape == want.shape
+    assert (off <= tol).all(), f"largest error {float((off / tol).max()):.2f} of the tolerance at {int((off / tol).argmax())}"
+
+
+SIZES = [(1, 32, 1), (1, 64, 16), (1, 2560, 9728), (2, 512, 257), (3, 544, 40), (5, 4096, 33), (15, 96, 64), (16, 5120, 512), (17, 160, 48),
+         (31, 1056, 129), (32, 2816, 130), (33, 1024, 1000), (47, 8192, 96), (64, 992, 256), (65, 288, 300), (96, 4096, 255),
+         (127, 480, 513), (128, 1024, 768), (129, 768, 384), (200, 9728, 320), (255, 256, 256), (256, 512, 512), (257, 2016, 259), (300, 32, 700),
+         (333, 2816, 1001), (511, 1280, 1280), (640, 736, 2050), (1025, 544, 1030)]
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("rows,k,n", SIZES)
+def test_product(rows, k, n, fmt):
+    dtype = (torch.bfloat16, torch.float16, torch.float32)[(rows + n) % 3]
+    w, ws = _weight(n, n, k)
+    codes, scales = nq.mx_quantize(_random(rows, rows, k, dtype=torch.float32), fmt)
+    bias = _random(k, n, dtype=dtype, spread=False) if rows % 2 else None
+    y = nq.mx_linear_quantized(codes, scales, w, ws, bias, dtype)
+    _check_product(y, (codes, scales), (w, ws), bias, dtype)
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("dt", DT)
+@pytest.mark.parametrize("rows,k,n", [(1, 32, 5), (1, 2560, 1000), (1, 25600, 64), (2, 992, 130), (4, 4096, 48), (7, 1056, 512), (16, 2048, 31),
+                                      (19, 5120, 160), (130, 1536, 257), (520, 768, 300)])
+def test_linear_quantises_as_quantize_does(rows, k, n, dt, fmt):
+    """The bits of mx_quantize and mx_linear_quantized wherever one kernel runs both, the definition's values everywhere."""
+    dtype = DT[dt]
+    w, ws = _weight(n, n, k)
+    x = _random(rows, rows, k, dtype=dtype)
+    bias = _random(k, n, dtype=dtype, spread=False) if rows % 2 else None
+    y = nq.mx_linear(x, w, ws, bias, activations=fmt)
+    codes, scales = mx.quantize(x, fmt)
+    _check_product(y, (codes, scales), (w, ws), bias, dtype)
+    again = nq.mx_linear_quantized(codes.cuda(), scales.cuda(), w, ws, bias, dtype)
+    assert torch.equal(y, again)
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("rows", [1, 16, 40, 100, 300])
+def test_every_code_and_wide_scales_in_a_product(rows, fmt):
+    """Codes at random, every one of both types among them, scales over most of their range: the pairing of codes and scales
+    along k shows in every value."""
+    g = _gen(rows)
+    k, n = 1184, 272
+    w = torch.randint(0, 256, (n, k // 2), device="cuda", generator=g, dtype=torch.uint8)
+    ws = torch.randint(100, 150, (n, k // 32), device="cuda", generator=g, dtype=torch.uint8)
+    if fmt == "mxfp4":
+        codes = torch.randint(0, 256, (rows, k // 2), device="cuda", generator=g, dtype=torch.uint8)
+    else:
+        codes = torch.randint(0, 254, (rows, k), device="cuda", generator=g, dtype=torch.uint8)
+        codes = torch.where(codes >= 127, codes + 1, codes)                 # without the two NaN codes
+        codes = torch.where(codes == 255, 0, codes)
+    scales = torch.randint(100, 150, (rows, k // 32), device="cuda", generator=g, dtype=torch.uint8)
+    y = nq.mx_linear_quantized(codes, scales, w, ws, None, torch.float32)
+    _check_product(y, (codes, scales), (w, ws), None, torch.float32)
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("rows,k,n", [(1, 544, 40), (20, 1056, 200), (70, 800, 300), (300, 2080, 520)])
+def test_one_block_at_a_time(rows, k, n, fmt):
+    """x has values in one block only: a sum takes that block's products, whole, and nothing else's."""
+    w, ws = _weight(3, n, k)
+    for b in sorted({0, 1, 3, k // 64, k // 32 - 2, k // 32 - 1}):
+        x = torch.zeros(rows, k, device="cuda")
+        x[:, 32 * b:32 * b + 32] = _random(b, rows, 32, dtype=torch.float32)
+        codes, scales = nq.mx_quantize(x, fmt)
+        y = nq.mx_linear_quantized(codes, scales, w, ws, None, torch.float32)
+        _check_product(y, (codes, scales), (w, ws), None, torch.float32)
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("rows", [1, 9, 50, 200, 400])
+def test_nan_stays_in_its_rows(rows, fmt):
+    """A block of NaN in a row of x makes that row of y NaN, one in a weight row that column; the rest is as without."""
+    k, n = 1120, 300
+    w, ws = _weight(5, n, k)
+    x = _random(6, rows, k)
+    clean = nq.mx_linear(x, w, ws, activations=fmt)
+    for at in (0, k // 2, k - 1):
+        bad = x.clone()
+        bad[rows // 2, at] = float("inf")
+        y = nq.mx_linear(bad, w, ws, activations=fmt)
+        keep = torch.arange(rows, device="cuda") != rows // 2
+        assert torch.isnan(y[rows // 2]).all() and torch.equal(y[keep], clean[keep])
+        wsb = ws.clone()
+        wsb[n - 1, at // 32] = 255
+        y = nq.mx_linear(x, w, wsb, activations=fmt)
+        assert torch.isnan(y[:, n - 1]).all() and torch.equal(y[:, :n - 1], clean[:, :n - 1])
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("rows", [1, 3, 24, 150, 270])
+def test_rows_do_not_depend_on_their_neighbours(rows, fmt):
+    """Results land in their own rows and nowhere else: memory behind y and between its ends stays."""
+    k, n = 672, 132
+    w, ws = _weight(7, n, k)
+    codes, scales = nq.mx_quantize(_random(8, rows, k), fmt)
+    y = nq.mx_linear_quantized(codes, scales, w, ws)
+    room = torch.full((rows * n + 4096,), 3.0, dtype=torch.bfloat16, device="cuda")
+    out = room[2048:2048 + rows * n]
+    _lib.check_mx(_lib.mx_lib().nqx_linear_quantized(codes.data_ptr(), scales.data_ptr(), w.data_ptr(), ws.data_ptr(), None, out.data_ptr(), rows, n,
+                                                     k, 1, FORMATS.index(fmt), torch.cuda.current_stream().cuda_stream))
+    torch.cuda.synchronize()
+    assert torch.equal(out.view(rows, n), y) and (room[:2048] == 3).all() and (room[2048 + rows * n:] == 3).all()
+
+
+def test_views_of_a_product():
+    w, ws = _weight(9, 96, 256)
+    wide = _random(10, 40, 1024)
+    for x in (wide[:, 256:512], wide[:, 1:257], wide[:3, 512:768], wide.t()[:256].t(), wide.view(4, 10, 1024)[:, ::3, :256]):
+        assert torch.equal(nq.mx_linear(x, w, ws), nq.mx_linear(x.contiguous(), w, ws))
+    flat = torch.empty(96 * 128 + 8, dtype=torch.uint8, device="cuda")
+    off = flat[3:3 + 96 * 128].view(96, 128)
+    off.copy_(w)
+    x = wide[:, :256].contiguous()
+    assert torch.equal(nq.mx_linear(x, off, ws), nq.mx_linear(x, w, ws))
+    s_off = torch.empty(96 * 8 + 1, dtype=torch.uint8, device="cuda")[1:].view(96, 8)
+    s_off.copy_(ws)
+    assert torch.equal(nq.mx_linear(x, w, s_off), nq.mx_linear(x, w, ws))
+    assert torch.equal(nq.mx_linear(x, w.t().contiguous().t(), ws), nq.mx_linear(x, w, ws))
+    b = _random(3, 97)[1:]
+    assert torch.equal(nq.mx_linear(x, w, ws, b), nq.mx_linear(x, w, ws, b.clone()))
+
+
+# ---- norm, SiLU: fp32 in front of the rounding ----------------------------------------------------------------------------
+def _check_rounded(packed, y, fmt, near, least=0.0):
+    """codes and scales of values that the kernel has in fp32 to within `near` of y, relative (or `least`): the scale is that of
+    such values, and every element is off by half a step at most, and what the value was off."""
+    got, e = mx.values(*packed), packed[1].cpu().to(torch.int64) - 127
+    largest = y.abs().unflatten(-1, (-1, 32)).amax(-1)
+    low = mx.scale_exponents((largest * (1 - near) - least).clamp_min(0), fmt)
+    high = mx.scale_exponents(largest * (1 + near) + least, fmt)
+    assert ((low <= e) & (e <= high)).all()
+    tol = mx.half_steps(y.abs() * (1 + near) + least, e, fmt) + y.abs() * near + least
+    off = (got - y).abs()
+    assert (off <= tol).all(), float((off / tol).max())
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("dt", DT)
+@pytest.mark.parametrize("rows,k", [(1, 32), (3, 64), (5, 544), (1, 4096), (17, 2048), (2, 2080), (33, 5120), (4, 9728), (3, 16384), (700, 512)])
+def test_add_rmsnorm(rows, k, dt, fmt):
+    t, eps = DT[dt], 1e-6
+    x, delta = _random(k, rows, k, dtype=t), _random(k + 1, rows, k, dtype=t, spread=False)
+    weight = (1 + 0.1 * _random(k + 2, k, dtype=torch.float32, spread=False)).to(t)
+    codes, scales, total = nq.mx_add_rmsnorm(x, delta, weight, eps, fmt)
+    assert torch.equal(total, x + delta)
+    s = total.cpu().double()
+    y = s / torch.sqrt((s * s).mean(-1, keepdim=True) + eps) * weight.cpu().double()
+    # the mean of squares: at most 64 additions of a lane, 6 of a wave, 4 of the workgroup, a square and a division, halved by
+    # the root; root, reciprocal and two products behind it
+    _check_rounded((codes, scales), y, fmt, ((64 + 6 + 4 + 2) / 2 + 5) * U * 1.01)
+    c2, s2, same = nq.mx_add_rmsnorm(total, None, weight, eps, fmt)
+    assert same is total and torch.equal(c2, codes) and torch.equal(s2, scales)
+
+
+def test_add_rmsnorm_views_and_aliases():
+    wide = _random(1, 12, 1024)
+    weight = _random(2, 256, spread=False)
+    x, delta = wide[:, :256], wide[:, 512:768]
+    want = nq.mx_add_rmsnorm(x.contiguous(), delta.contiguous(), weight)
+    for got in (nq.mx_add_rmsnorm(x, delta, weight), nq.mx_add_rmsnorm(x.contiguous(), delta, weight),
+                nq.mx_add_rmsnorm(x.reshape(3, 4, 256), delta.reshape(3, 4, 256), weight)):
+        assert all(torch.equal(a.reshape(b.shape), b) for a, b in zip(got, want))
+    off = torch.empty(257, dtype=torch.bfloat16, device="cuda")[1:]
+    off.copy_(weight)
+    assert all(torch.equal(a, b) for a, b in zip(nq.mx_add_rmsnorm(x, delta, off), want))
+    # the C ABI in place: total is x, or delta
+    for which in (0, 1):
+        a, b = x.contiguous(), delta.contiguous()
+        codes, scales = torch.empty(12, 256, dtype=torch.uint8, device="cuda"), torch.empty(12, 8, dtype=torch.uint8, device="cuda")
+        to = (a, b)[which]
+        _lib.check_mx(_lib.mx_lib().nqx_add_rmsnorm(a.data_ptr(), 256, b.data_ptr(), 256, weight.data_ptr(), to.data_ptr(), codes.data_ptr(),
+                                                    scales.data_ptr(), 12, 256, 1e-6, 1, 1, torch.cuda.current_stream().cuda_stream))
+        assert torch.equal(to, want[2]) and torch.equal(codes, want[0]) and torch.equal(scales, want[1])
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+def test_norm_of_odd_rows(fmt):
+    """Rows of zeros, of the type's largest values, with an infinity, with a NaN."""
+    weight = torch.ones(96, dtype=torch.bfloat16, device="cuda")
+    x = torch.zeros(5, 96, dtype=torch.bfloat16, device="cuda")
+    x[1] = 1e18
+    x[2] = _random(1, 96)
+    x[2, 40] = float("inf")
+    x[3, 95] = float("nan")
+    x[4] = 1.0
+    codes, scales, _ = nq.mx_add_rmsnorm(x, torch.zeros_like(x), weight, 1e-6, fmt)
+    v = mx.values(codes, scales)
+    assert (v[0] == 0).all() and (v[1] == 1).all() and (v[4] == 1).all()
+    # infinity: the other values are divided by it, its own block is NaN as 0 * inf is
+    assert (v[2, :32] == 0).all() and torch.isnan(v[2, 32:64]).all() and (v[2, 64:] == 0).all()
+    assert torch.isnan(v[3]).all()
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("dt", DT)
+@pytest.mark.parametrize("rows,k", [(1, 32), (7, 9728), (5, 96), (130, 1024), (2, 12288)])
+def test_silu_mul(rows, k, dt, fmt):
+    t = DT[dt]
+    both = torch.cat([4 * _random(k, rows, k, dtype=torch.float32, spread=False), _random(k + 1, rows, k, dtype=torch.float32)], -1).to(t)
+    gate, up = both[:, :k], both[:, k:]
+    packed = nq.mx_silu_mul(gate, up, fmt)
+    g, u = gate.cpu().double(), up.cpu().double()
+    # exp to within two steps of fp32 (four half steps), 1 + it, the division or a reciprocal of one step and its product, the product
+    _check_rounded(packed, g / (1 + torch.exp(-g)) * u, fmt, 12 * U, 2.0 ** -140)
+    again = nq.mx_silu_mul(gate.contiguous(), up.contiguous(), fmt)
+    assert torch.equal(packed[0], again[0]) and torch.equal(packed[1], again[1])
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+def test_silu_far_out(fmt):
+    """Gates whose exponential overflows or vanishes, infinities and NaN."""
+    g = torch.tensor([-1e4, -200.0, -120.0, -90.0, -88.0, -60.0, -20.0, -1.0, 0.0, 1.0, 20.0, 60.0, 90.0, 200.0, 1e4, 3e38], device="cuda")
+    gate = torch.stack([v.expand(32) for v in g] + [torch.full((32,), float(s), device="cuda") for s in ("inf", "-inf", "nan")])
+    up = torch.ones_like(gate)
+    codes, scales = nq.mx_silu_mul(gate, up, fmt)
+    v, e = mx.values(codes, scales)[:, 0], scales.cpu().to(torch.int64)[:, 0] - 127
+    want = (gate.cpu().double() * torch.sigmoid(gate.cpu().double()))[:, 0]
+    assert torch.isnan(v[-3:]).all()                   # inf, and -inf * 0, and NaN
+    half = mx.half_steps(want[:-3].unsqueeze(1).expand(-1, 32), e[:-3].unsqueeze(1), fmt)[:, 0]
+    assert ((v[:-3] - want[:-3]).abs() <= half + want[:-3].abs() * 12 * U + 2.0 ** -120).all()
+
+
+# ---- as they are used -----------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("rows", [1, 6, 40, 200])
+def test_a_feed_forward_of_them(rows, fmt):
+    """residual + norm -> gate | up -> SiLU -> down, every step against the definition on what the step before left."""
+    hidden, inter = 512, 1408
+    torch.manual_seed(rows)
+    gate_up = nq.MXLinear.from_linear(torch.nn.Linear(hidden, 2 * inter, bias=False, device="cuda", dtype=torch.bfloat16), fmt)
+    down = nq.MXLinear.from_linear(torch.nn.Linear(inter, hidden, device="cuda", dtype=torch.bfloat16), fmt)
+    residual, delta, weight = _random(1, rows, hidden), _random(2, rows, hidden), _random(3, hidden, spread=False)
+    codes, scales, residual = nq.mx_add_rmsnorm(residual, delta, weight, 1e-6, fmt)
+    both = gate_up((codes, scales))
+    _check_product(both, (codes, scales), (gate_up.weight, gate_up.weight_scales), None, torch.bfloat16)
+    act = nq.mx_silu_mul(both[:, :inter], both[:, inter:], fmt)
+    g, u = both[:, :inter].cpu().double(), both[:, inter:].cpu().double()
+    _check_rounded(act, g / (1 + torch.exp(-g)) * u, fmt, 12 * U, 2.0 ** -140)
+    y = down(act)
+    _check_product(y, act, (down.weight, down.weight_scales), down.bias, torch.bfloat16)
+    # a tensor in place of (codes, scales) is quantised on the way
+    x = _random(4, 2, rows, hidden)
+    assert torch.equal(gate_up(x).view(2 * rows, -1), gate_up(nq.mx_quantize(x.view(-1, hidden), fmt)))
+
+
+def test_module_keeps_its_weights():
+    lin = torch.nn.Linear(320, 77, device="cuda")
+    m = nq.MXLinear.from_linear(lin, "mxfp4", torch.float16)
+    w = mx.quantize(lin.weight, "mxfp4")
+    _equal_packed((m.weight, m.weight_scales), w)
+    assert m.bias.dtype == torch.float16
+    other = nq.MXLinear(320, 77, True, "mxfp4", "cuda", torch.float16)
+    other.load_state_dict(m.state_dict())
+    x = _random(1, 5, 320, dtype=torch.float16)
+    assert torch.equal(other(x), m(x))
+
+
+def test_streams_and_graphs():
+    """A linear on another stream, and two captured graphs of different sizes replayed in turn with eager work between."""
+    w, ws = _weight(1, 640, 1088)
+    xs = [_random(i, r, 1088) for i, r in enumerate((1, 5, 70, 300))]
+    want = [nq.mx_linear(x, w, ws) for x in xs]
+    torch.cuda.synchronize()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        got = [nq.mx_linear(x, w, ws) for x in xs]
+    torch.cuda.current_stream().wait_stream(side)
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+    norm_w = _random(9, 1088, spread=False)
+    graphs = []
+    for x in xs:
+        static = x.clone()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            codes, scales, total = nq.mx_add_rmsnorm(static, static, norm_w)
+            out = (nq.mx_linear(total, w, ws), nq.mx_linear_quantized(codes, scales, w, ws))
+        graphs.append((graph, static, out))
+    for turn in range(3):
+        fresh = [_random(20 + turn, *x.shape) for x in xs]
+        for (graph, static, _), x in zip(graphs, fresh):
+            static.copy_(x)
+            graph.replay()
+        torch.cuda.synchronize()
+        for (_, _, out), x in zip(graphs, fresh):
+            codes, scales, total = nq.mx_add_rmsnorm(x, x, norm_w)
+            assert torch.equal(out[0], nq.mx_linear(total, w, ws)) and torch.equal(out[1], nq.mx_linear_quantized(codes, scales, w, ws))
+
+
+def test_past_32_bits():
+    """Outputs and inputs of more than 2^32 values."""
+    base = _random(1, 1, 32)
+    x = base.expand((1 << 27) + 5, 32)                        # one row in memory
+    codes, scales = nq.mx_quantize(x, "mxfp8")
+    one = nq.mx_quantize(base, "mxfp8")
+    assert torch.equal(codes[-9:], one[0].expand(9, 32)) and torch.equal(codes[::1 << 20], one[0].expand(129, 32))
+    assert bool((scales == one[1]).all())
+    back = nq.mx_dequantize(codes, scales, torch.bfloat16)
+    assert torch.equal(back[-3:], nq.mx_dequantize(*one).expand(3, 32))
+    del x, codes, scales, back
+    rows, n = 70000, 61500
+    w, ws = _weight(2, n, 32)
+    x = _random(3, rows, 32)
+    y = nq.mx_linear(x, w, ws)
+    for r in (0, 34919, 34920, rows - 1):
+        assert torch.equal(y[r:r + 1], nq.mx_linear(x[r:r + 1].clone(), w, ws))
+    del y
+    torch.cuda.empty_cache()
