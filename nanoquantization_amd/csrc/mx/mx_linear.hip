@@ -19,7 +19,15 @@ int check_operands(const char* fn, const uint8_t* weight, const uint8_t* weight_
     return NQX_OK;
 }
 
-int product(const Product& p, hipStream_t stream) { return skinny_product(p, stream); }
+// Which kernel runs a product: 0 the one that streams the weight, else the size of a tile.
+int form_of(int64_t rows, int64_t n, int64_t k, int format) {
+    if (rows <= 64 || k > ((int64_t)1 << 22)) return 0;      // byte offsets in a tile are 32 bits
+    return cdiv(rows, 256) * cdiv(n, 256) >= 192 ? 256 : 128;
+}
+int product(const Product& p, hipStream_t stream) {
+    const int form = form_of(p.rows, p.n, p.k, p.format);
+    return form ? tiles_product(p, form, stream) : skinny_product(p, stream);
+}
 
 // Where nqx_linear keeps the quantised x: codes, then scales.
 int64_t scales_at(int64_t rows, int64_t k, int format) { return rows * code_bytes(k, format); }
@@ -63,5 +71,6 @@ extern "C" int nqx_linear(const void* x, int64_t x_stride, const uint8_t* weight
 
 extern "C" const char* nqx_linear_form(int64_t rows, int64_t n, int64_t k, int dtype, int format, int) {
     if (check_product("nqx_linear_form", rows, n, k, dtype, format) || rows == 0 || n == 0) return "";
-    return "mx_skinny_kernel";
+    const int form = form_of(rows, n, k, format);
+    return form == 256 ? "mx_tiles_kernel 256 x 256" : form == 128 ? "mx_tiles_kernel 128 x 128" : "mx_skinny_kernel";
 }

@@ -48,5 +48,6 @@ __device__ __forceinline__ void store_sums(f32x4 v, typename T::elem* y, const t
 }
 
 int skinny_product(const Product& p, hipStream_t stream);
+int tiles_product(const Product& p, int tile, hipStream_t stream);
 
 }  // namespace nqx
