@@ -27,6 +27,15 @@ __device__ __forceinline__ f32x4 mfma(u32x4 w, u32x4 x0, u32x4 x1, f32x4 c, uint
     return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, b, c, 4, FORMAT == NQX_FP4 ? 4 : 0, 0, (int)w_scale, 0, (int)x_scale);
 }
 
+// e2m1 with e2m1: 32 weight rows x 32 rows of x over 64 values.  Lane l has row l % 32 and one block; with h = l / 32 the result is
+// column l % 32, weight rows 8 q + 4 h .. 8 q + 4 h + 3 in the elements 4 q .. 4 q + 3.  BYTE: which byte of the words holds the scales.
+template <int BYTE>
+__device__ __forceinline__ f32x16 mfma32(u32x4 w, u32x4 x, f32x16 c, uint32_t w_scale, uint32_t x_scale) {
+    const i32x8 a = {(int)w[0], (int)w[1], (int)w[2], (int)w[3], 0, 0, 0, 0};
+    const i32x8 b = {(int)x[0], (int)x[1], (int)x[2], (int)x[3], 0, 0, 0, 0};
+    return __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(a, b, c, 4, 4, BYTE, (int)w_scale, BYTE, (int)x_scale);
+}
+
 // Four consecutive values of a row of y, columns n .. n + 3 of which those below N exist.
 template <typename T>
 __device__ __forceinline__ void store_sums(f32x4 v, typename T::elem* y, const typename T::elem* bias, int64_t row, int64_t n,
