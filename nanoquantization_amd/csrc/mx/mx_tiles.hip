@@ -37,7 +37,7 @@ struct Tiles {
     static_assert(kLds <= 160 * 1024, "");
 };
 
-template <typename T, int FORMAT, int S>
+template <typename T, int FORMAT, int S, bool BIAS>
 __global__ __launch_bounds__(256, (S == 256 ? 1 : 2)) void mx_tiles_kernel(
     const uint8_t* __restrict__ x, const uint8_t* __restrict__ xs, const uint8_t* __restrict__ w, const uint8_t* __restrict__ ws,
     const typename T::elem* __restrict__ bias, typename T::elem* __restrict__ y, int rows, int N, int blocks, int words, int x_tiles,
@@ -156,15 +156,32 @@ __global__ __launch_bounds__(256, (S == 256 ? 1 : 2)) void mx_tiles_kernel(
         __builtin_amdgcn_sched_barrier(0);
     };
 
-    // ---- before the first chunk ----
+    // ---- before the first chunk: requests first, what the waves bring themselves behind them ----
+    if (!part) {
+#pragma unroll
+        for (int q = 0; q < G::kLoads; ++q) load_w(q, 0), load_x(q, 0);
+        if (!kFour) {
+#pragma unroll
+            for (int q = 0; q < G::kLoads; ++q) load_x(q, 1);
+        }
+    }
+    // what goes out behind the barrier of a chunk that does not exist
+    if (kFour) {
+#pragma unroll
+        for (int q = 0; q < G::kLoads; ++q) load_w(q, 1), load_x(q, 1);
+    } else {
+#pragma unroll
+        for (int q = 0; q < G::kLoads / 2; ++q) load_w(q, 1);
+    }
     if (whole >= 4) {
-        load_scales(0);
+        if (words) bring_scales(0, 0);
+        else load_scales(0);
     } else {
 #pragma unroll
         for (int i = 0; i < 6; ++i)
             if (i < 2 * whole) sw[i >> 2][i & 3] = four_bytes(swp + 4 * i), sx[i >> 2][i & 3] = four_bytes(sxp + 4 * i);
     }
-    store_scales(0);
+    if (!words || whole < 4) store_scales(0);
     if (part) {
         sw[0][0] = part_bytes(swp, 0), sw[0][1] = part_bytes(swp, 4), sx[0][0] = part_bytes(sxp, 0), sx[0][1] = part_bytes(sxp, 4);
         store_scales(1);
@@ -181,21 +198,6 @@ __global__ __launch_bounds__(256, (S == 256 ? 1 : 2)) void mx_tiles_kernel(
                 *reinterpret_cast<u32x4*>(s_mem + G::kX + h * G::kPart + to) = v;
             }
         }
-    } else {
-#pragma unroll
-        for (int q = 0; q < G::kLoads; ++q) load_w(q, 0), load_x(q, 0);
-        if (!kFour) {
-#pragma unroll
-            for (int q = 0; q < G::kLoads; ++q) load_x(q, 1);
-        }
-    }
-    // what goes out behind the barrier of a chunk that does not exist
-    if (kFour) {
-#pragma unroll
-        for (int q = 0; q < G::kLoads; ++q) load_w(q, 1), load_x(q, 1);
-    } else {
-#pragma unroll
-        for (int q = 0; q < G::kLoads / 2; ++q) load_w(q, 1);
     }
     hand_over();
     // the scales of four chunks, three to four chunks ahead; through registers those loaded a chunk ago
@@ -336,36 +338,19 @@ __global__ __launch_bounds__(256, (S == 256 ? 1 : 2)) void mx_tiles_kernel(
     constexpr int kQ = R * R / 256, kV = 16 / sizeof(E), kPitch = TW / 2 * sizeof(E) + 16;
     static_assert(4 * R * kPitch <= G::kLds, "");
     const int64_t n_wave = n0 + wm * (TW / 2), m_wave = m0 + wn * (TX / 2);
-    f32x4 add[WT][kQ];
-#pragma unroll
-    for (int i = 0; i < WT; ++i)
-#pragma unroll
-        for (int q = 0; q < kQ; ++q)
+    const bool full = n_wave + TW / 2 <= N;      // and else a row ends in the tile
+    const auto value = [&](int i, int j, int q) {
+        f32x4 v = {acc[i][j][4 * q], acc[i][j][4 * q + 1], acc[i][j][4 * q + 2], acc[i][j][4 * q + 3]};
+        if constexpr (BIAS) {
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
                 const int64_t n = n_wave + i * R + 8 * q + 4 * part_of + e;
-                add[i][q][e] = bias && n < N ? T::to_f32(bias[n]) : 0.f;
+                v[e] += T::to_f32(bias[n < N ? n : N - 1]);
             }
-    const auto value = [&](int i, int j, int q) {
-        f32x4 v;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) v[e] = acc[i][j][4 * q + e] + add[i][q][e];
+        }
         return v;
     };
-    if (N % kV != 0) {
-#pragma unroll
-        for (int j = 0; j < XT; ++j)
-#pragma unroll
-            for (int i = 0; i < WT; ++i)
-#pragma unroll
-                for (int q = 0; q < kQ; ++q) {
-                    const int64_t m = m_wave + j * R + row, n = n_wave + i * R + 8 * q + 4 * part_of;
-                    if (m < rows && n < N) store_sums<T>(value(i, j, q), y, nullptr, m, n, N);
-                }
-        return;
-    }
-    __builtin_amdgcn_s_waitcnt(0x0070);      // nothing is on its way to LDS any more, and nobody reads a stage
-    __syncthreads();
+    hand_over();             // nobody reads a chunk any more, and no request, the empty ones among them, is on its way to LDS
     unsigned char* s_out = s_mem + wave * R * kPitch;
 #pragma unroll
     for (int j = 0; j < XT; ++j) {
@@ -379,28 +364,36 @@ __global__ __launch_bounds__(256, (S == 256 ? 1 : 2)) void mx_tiles_kernel(
                 else *reinterpret_cast<u32x2*>(to) = u32x2{T::pack2(v[0], v[1]), T::pack2(v[2], v[3])};
             }
         __builtin_amdgcn_wave_barrier();
-        constexpr int kLanes = TW / 2 / kV;  // of a row
+        constexpr int kLanes = TW / 2 / kV;      // of a row
 #pragma unroll
         for (int q = 0; q < R * kLanes / 64; ++q) {
             const int r = (q * 64 + lane) / kLanes, c = (q * 64 + lane) % kLanes;
-            const u32x4 v = *reinterpret_cast<const u32x4*>(s_out + r * kPitch + c * 16);
+            const unsigned char* from = s_out + r * kPitch + c * 16;
             const int64_t m = m_wave + j * R + r, n = n_wave + c * kV;
-            if (m < rows && n < N) *reinterpret_cast<u32x4*>(y + m * N + n) = v;
+            const u32x4 v = *reinterpret_cast<const u32x4*>(from);
+            if (m >= rows) continue;
+            if (full) {
+                __builtin_memcpy(y + m * N + n, &v, 16);     // any address of the type
+            } else {
+#pragma unroll 1
+                for (int e = 0; e < kV; ++e)
+                    if (n + e < N) y[m * N + n + e] = reinterpret_cast<const E*>(from)[e];
+            }
         }
         __builtin_amdgcn_wave_barrier();
     }
 }
 
-template <typename T, int FORMAT, int S>
+template <typename T, int FORMAT, int S, bool BIAS>
 hipError_t launch(const Product& p, hipStream_t stream) {
     using G = Tiles<FORMAT, S>;
     using E = typename T::elem;
     const int x_tiles = (int)cdiv(p.rows, S), w_tiles = (int)cdiv(p.n, S);
-    const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(&mx_tiles_kernel<T, FORMAT, S>),
+    const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(&mx_tiles_kernel<T, FORMAT, S, BIAS>),
                                              hipFuncAttributeMaxDynamicSharedMemorySize, G::kLds);
     if (e != hipSuccess) return e;
     const unsigned grid = (unsigned)(cdiv((int64_t)x_tiles * w_tiles, 8) * 8);
-    mx_tiles_kernel<T, FORMAT, S><<<grid, G::kThreads, G::kLds, stream>>>(
+    mx_tiles_kernel<T, FORMAT, S, BIAS><<<grid, G::kThreads, G::kLds, stream>>>(
         p.x, p.xs, p.w, p.ws, static_cast<const E*>(p.bias), static_cast<E*>(p.y), (int)p.rows, (int)p.n, (int)(p.k / kBlock),
         p.k / kBlock % 4 == 0 && ((reinterpret_cast<uintptr_t>(p.ws) | reinterpret_cast<uintptr_t>(p.xs)) & 3) == 0, x_tiles, w_tiles);
     return hipGetLastError();
@@ -413,7 +406,8 @@ int tiles_product(const Product& p, int tile, hipStream_t stream) {
     by_type(p.dtype, p.format, [&](auto t, auto f) {
         using T = decltype(t);
         constexpr int F = decltype(f)::value;
-        e = tile == 256 ? launch<T, F, 256>(p, stream) : launch<T, F, 128>(p, stream);
+        if (p.bias) e = tile == 256 ? launch<T, F, 256, true>(p, stream) : launch<T, F, 128, true>(p, stream);
+        else e = tile == 256 ? launch<T, F, 256, false>(p, stream) : launch<T, F, 128, false>(p, stream);
     });
     return e == hipSuccess ? NQX_OK : refuse(NQX_ERR_HIP, "mx_tiles_kernel: HIP error %d (%s)", (int)e, hipGetErrorString(e));
 }
