@@ -174,8 +174,8 @@ MX_SYMBOLS = {
     "nqx_last_error": (ctypes.c_char_p, []),
     "nqx_quantize": (_int, [_vp, _i64, _vp, _vp, _i64, _i64, _int, _int, _vp]),
     "nqx_dequantize": (_int, [_vp, _vp, _vp, _i64, _i64, _int, _int, _vp]),
-    "nqx_linear_quantized": (_int, [_vp] * 6 + [_i64] * 3 + [_int, _int, _vp]),
-    "nqx_linear_workspace_bytes": (_sz, [_i64] * 3 + [_int, _int]),
+    "nqx_linear_quantized": (_int, [_vp] * 6 + [_i64] * 3 + [_int, _int, _vp, _sz, _vp]),
+    "nqx_linear_workspace_bytes": (_sz, [_i64] * 3 + [_int] * 3),
     "nqx_linear": (_int, [_vp, _i64] + [_vp] * 4 + [_i64] * 3 + [_int, _int, _vp, _sz, _vp]),
     "nqx_linear_form": (ctypes.c_char_p, [_i64] * 3 + [_int] * 3),
     "nqx_add_rmsnorm": (_int, [_vp, _i64, _vp, _i64] + [_vp] * 4 + [_i64, _i64, _f32, _int, _int, _vp]),

@@ -144,7 +144,7 @@ at::Tensor mx_linear(const at::Tensor& x, const at::Tensor& weight, const at::Te
     if (y.numel() == 0) return y;
     const Rows r = rows_of(x);
     const at::Tensor w = dense16(weight), ws = weight_scales.contiguous();
-    const size_t bytes = nqx_linear_workspace_bytes(r.rows, n, k, d, f);
+    const size_t bytes = nqx_linear_workspace_bytes(r.rows, n, k, d, f, 0);
     const at::Tensor space = bytes ? at::empty({(int64_t)bytes}, w.options()) : at::Tensor();
     check_status(nqx_linear(r.t.data_ptr(), r.stride, w.data_ptr<uint8_t>(), ws.data_ptr<uint8_t>(), b.defined() ? b.data_ptr() : nullptr,
                             y.data_ptr(), r.rows, n, k, d, f, bytes ? space.data_ptr() : nullptr, bytes, stream_of(x)),
@@ -169,8 +169,12 @@ at::Tensor mx_linear_quantized(const at::Tensor& codes, const at::Tensor& scales
     const at::Tensor b = dense_bias(bias, codes, n, dtype);
     if (y.numel() == 0) return y;
     const at::Tensor c = dense16(codes), s = scales.contiguous(), w = dense16(weight), ws = weight_scales.contiguous();
+    const int64_t rows = y.numel() / n;
+    const size_t bytes = nqx_linear_workspace_bytes(rows, n, p.k, d, p.format, 1);
+    const at::Tensor space = bytes ? at::empty({(int64_t)bytes}, w.options()) : at::Tensor();
     check_status(nqx_linear_quantized(c.data_ptr<uint8_t>(), s.data_ptr<uint8_t>(), w.data_ptr<uint8_t>(), ws.data_ptr<uint8_t>(),
-                                      b.defined() ? b.data_ptr() : nullptr, y.data_ptr(), y.numel() / n, n, p.k, d, p.format, stream_of(codes)),
+                                      b.defined() ? b.data_ptr() : nullptr, y.data_ptr(), rows, n, p.k, d, p.format,
+                                      bytes ? space.data_ptr() : nullptr, bytes, stream_of(codes)),
                  "nqx_linear_quantized");
     return y;
 }

@@ -19,36 +19,64 @@ int check_operands(const char* fn, const uint8_t* weight, const uint8_t* weight_
     return NQX_OK;
 }
 
-// Which kernel runs a product: 0 the one that streams the weight, else the size of a tile.
-int form_of(int64_t rows, int64_t n, int64_t k, int format) {
-    if (rows <= 64 || k > ((int64_t)1 << 22)) return 0;      // byte offsets in a tile are 32 bits
-    return cdiv(rows, 256) * cdiv(n, 256) >= 192 ? 256 : 128;
+enum Form { kSkinny, kStream, kTiles128, kTiles256 };
+
+// Which kernel runs a product.
+Form form_of(int64_t rows, int64_t n, int64_t k) {
+    if (k > ((int64_t)1 << 22)) return kSkinny;              // byte offsets in a tile are 32 bits
+    if (rows <= 128) return kStream;
+    return cdiv(rows, 256) * cdiv(n, 256) >= 192 ? kTiles256 : kTiles128;
+}
+// Whether a linear quantises x in the product's own kernel.
+bool raw_of(int64_t rows, int64_t n, int64_t k, int format) {
+    return rows <= 16 && form_of(rows, n, k) == kStream && stream_raw_bytes(rows, n, k, format) <= 48 * 1024;
 }
 int product(const Product& p, hipStream_t stream) {
-    const int form = form_of(p.rows, p.n, p.k, p.format);
-    return form ? tiles_product(p, form, stream) : skinny_product(p, stream);
+    switch (form_of(p.rows, p.n, p.k)) {
+        case kTiles256: return tiles_product(p, 256, stream);
+        case kTiles128: return tiles_product(p, 128, stream);
+        case kStream: return stream_product(p, stream);
+        default: return skinny_product(p, stream);
+    }
 }
 
-// Where nqx_linear keeps the quantised x: codes, then scales.
-int64_t scales_at(int64_t rows, int64_t k, int format) { return rows * code_bytes(k, format); }
+// A call's workspace: the sums of a split product, the codes of x, the scales of x.
+struct Space {
+    size_t sums, codes, scales;
+    size_t bytes() const { return sums + codes + scales; }
+};
+Space space_of(int64_t rows, int64_t n, int64_t k, int format, bool quantised) {
+    Space s = {0, 0, 0};
+    if (rows == 0 || n == 0) return s;
+    if (form_of(rows, n, k) == kStream) s.sums = stream_sums_bytes(rows, n, k, format);
+    if (!quantised && !raw_of(rows, n, k, format)) s.codes = (size_t)(rows * code_bytes(k, format)), s.scales = (size_t)(rows * (k / kBlock));
+    return s;
+}
+int check_space(const char* fn, size_t wanted, const void* workspace, size_t bytes) {
+    if (wanted && (!workspace || !aligned16(workspace) || bytes < wanted))
+        return refuse(NQX_ERR_WORKSPACE, "%s: a 16-byte aligned workspace of %zu bytes is needed, got %zu", fn, wanted, workspace ? bytes : 0);
+    return NQX_OK;
+}
 
 }  // namespace
 
+extern "C" size_t nqx_linear_workspace_bytes(int64_t rows, int64_t n, int64_t k, int dtype, int format, int quantised) {
+    if (check_product("nqx_linear_workspace_bytes", rows, n, k, dtype, format)) return 0;
+    return space_of(rows, n, k, format, quantised != 0).bytes();
+}
+
 extern "C" int nqx_linear_quantized(const uint8_t* codes, const uint8_t* scales, const uint8_t* weight,
                                     const uint8_t* weight_scales, const void* bias, void* y, int64_t rows, int64_t n, int64_t k,
-                                    int dtype, int format, void* stream) {
+                                    int dtype, int format, void* workspace, size_t workspace_bytes, void* stream) {
     const char* fn = "nqx_linear_quantized";
     if (int s = check_product(fn, rows, n, k, dtype, format)) return s;
     if (rows == 0 || n == 0) return NQX_OK;
     if (!codes || !aligned16(codes) || !scales)
         return refuse(NQX_ERR_ARG, "%s: codes must be a 16-byte aligned device pointer, and scales not null", fn);
     if (int s = check_operands(fn, weight, weight_scales, y)) return s;
-    return product({codes, scales, weight, weight_scales, bias, y, rows, n, k, dtype, format}, static_cast<hipStream_t>(stream));
-}
-
-extern "C" size_t nqx_linear_workspace_bytes(int64_t rows, int64_t n, int64_t k, int dtype, int format) {
-    if (check_product("nqx_linear_workspace_bytes", rows, n, k, dtype, format) || rows == 0 || n == 0) return 0;
-    return (size_t)(scales_at(rows, k, format) + rows * (k / kBlock));
+    if (int s = check_space(fn, space_of(rows, n, k, format, true).bytes(), workspace, workspace_bytes)) return s;
+    return product({codes, scales, weight, weight_scales, bias, y, rows, n, k, dtype, format, static_cast<float*>(workspace)},
+                   static_cast<hipStream_t>(stream));
 }
 
 extern "C" int nqx_linear(const void* x, int64_t x_stride, const uint8_t* weight, const uint8_t* weight_scales, const void* bias,
@@ -59,18 +87,27 @@ extern "C" int nqx_linear(const void* x, int64_t x_stride, const uint8_t* weight
     if (rows == 0 || n == 0) return NQX_OK;
     if (int s = check_rows(fn, "x", x, x_stride, k, dtype)) return s;
     if (int s = check_operands(fn, weight, weight_scales, y)) return s;
-    const size_t wanted = nqx_linear_workspace_bytes(rows, n, k, dtype, format);
-    if (!workspace || !aligned16(workspace) || workspace_bytes < wanted)
-        return refuse(NQX_ERR_WORKSPACE, "%s: a 16-byte aligned workspace of %zu bytes is needed, got %zu", fn, wanted, workspace ? workspace_bytes : 0);
-    uint8_t* codes = static_cast<uint8_t*>(workspace);
-    uint8_t* scales = codes + scales_at(rows, k, format);
+    const Space space = space_of(rows, n, k, format, false);
+    if (int s = check_space(fn, space.bytes(), workspace, workspace_bytes)) return s;
     const hipStream_t st = static_cast<hipStream_t>(stream);
+    Product p = {nullptr, nullptr, weight, weight_scales, bias, y, rows, n, k, dtype, format, static_cast<float*>(workspace)};
+    if (!space.codes) {
+        p.raw = x, p.raw_stride = x_stride;
+        return product(p, st);
+    }
+    uint8_t* codes = static_cast<uint8_t*>(workspace) + space.sums;
+    uint8_t* scales = codes + space.codes;
     if (int s = quantize(x, x_stride, codes, scales, rows, k, dtype, format, st)) return s;
-    return product({codes, scales, weight, weight_scales, bias, y, rows, n, k, dtype, format}, st);
+    p.x = codes, p.xs = scales;
+    return product(p, st);
 }
 
-extern "C" const char* nqx_linear_form(int64_t rows, int64_t n, int64_t k, int dtype, int format, int) {
+extern "C" const char* nqx_linear_form(int64_t rows, int64_t n, int64_t k, int dtype, int format, int quantised) {
     if (check_product("nqx_linear_form", rows, n, k, dtype, format) || rows == 0 || n == 0) return "";
-    const int form = form_of(rows, n, k, format);
-    return form == 256 ? "mx_tiles_kernel 256 x 256" : form == 128 ? "mx_tiles_kernel 128 x 128" : "mx_skinny_kernel";
+    switch (form_of(rows, n, k)) {
+        case kTiles256: return "mx_tiles_kernel 256 x 256";
+        case kTiles128: return "mx_tiles_kernel 128 x 128";
+        case kStream: return !quantised && raw_of(rows, n, k, format) ? "mx_stream_kernel on x as it is" : "mx_stream_kernel";
+        default: return "mx_skinny_kernel";
+    }
 }

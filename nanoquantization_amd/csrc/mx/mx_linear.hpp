@@ -15,6 +15,9 @@ struct Product {
     void* y;
     int64_t rows, n, k;
     int dtype, format;
+    float* sums;                // what stream_sums_bytes asks for
+    const void* raw = nullptr;  // in place of x and xs: x of the call's type, rows raw_stride apart
+    int64_t raw_stride = 0;
 };
 
 // One matrix instruction: 16 weight rows x 16 rows of x over 128 values (four blocks).  Lane l has row l % 16 and, with
@@ -58,5 +61,10 @@ __device__ __forceinline__ void store_sums(f32x4 v, typename T::elem* y, const t
 
 int skinny_product(const Product& p, hipStream_t stream);
 int tiles_product(const Product& p, int tile, hipStream_t stream);
+int stream_product(const Product& p, hipStream_t stream);       // at most 128 rows, at most 16 of raw x
+int stream_splits(int64_t rows, int64_t n, int64_t k, int format);
+int stream_chunks(int chunks, int blocks, int splits);
+size_t stream_sums_bytes(int64_t rows, int64_t n, int64_t k, int format);
+int stream_raw_bytes(int64_t rows, int64_t n, int64_t k, int format);
 
 }  // namespace nqx

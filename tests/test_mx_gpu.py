@@ -275,8 +275,10 @@ def test_rows_do_not_depend_on_their_neighbours(rows, fmt):
     y = nq.mx_linear_quantized(codes, scales, w, ws)
     room = torch.full((rows * n + 4096,), 3.0, dtype=torch.bfloat16, device="cuda")
     out = room[2048:2048 + rows * n]
-    _lib.check_mx(_lib.mx_lib().nqx_linear_quantized(codes.data_ptr(), scales.data_ptr(), w.data_ptr(), ws.data_ptr(), None, out.data_ptr(), rows, n,
-                                                     k, 1, FORMATS.index(fmt), torch.cuda.current_stream().cuda_stream))
+    L = _lib.mx_lib()
+    space = torch.empty(max(16, L.nqx_linear_workspace_bytes(rows, n, k, 1, FORMATS.index(fmt), 1)), dtype=torch.uint8, device="cuda")
+    _lib.check_mx(L.nqx_linear_quantized(codes.data_ptr(), scales.data_ptr(), w.data_ptr(), ws.data_ptr(), None, out.data_ptr(), rows, n, k, 1,
+                                         FORMATS.index(fmt), space.data_ptr(), space.numel(), torch.cuda.current_stream().cuda_stream))
     torch.cuda.synchronize()
     assert torch.equal(out.view(rows, n), y) and (room[:2048] == 3).all() and (room[2048 + rows * n:] == 3).all()
 

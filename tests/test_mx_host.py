@@ -56,7 +56,7 @@ def test_c_abi_refuses_before_it_launches():
     assert dequantize(rows=0, y=None) == 0
 
     def product(codes=at, scales=at, w=at, ws=at, y=at, rows=4, n=64, k=64, dtype=1, fmt=1):
-        return L.nqx_linear_quantized(codes, scales, w, ws, None, y, rows, n, k, dtype, fmt, None)
+        return L.nqx_linear_quantized(codes, scales, w, ws, None, y, rows, n, k, dtype, fmt, at, 1 << 30, None)
 
     assert product(codes=None) == product(codes=at + 8) == product(scales=None) == product(w=at + 8) == product(ws=None) == 1
     assert product(y=None) == product(n=-1) == product(k=40) == 1
@@ -64,13 +64,19 @@ def test_c_abi_refuses_before_it_launches():
     assert product(rows=0, codes=None) == product(n=0, w=None) == 0
 
     def linear(x=at, stride=64, ws_bytes=1 << 20, space=at, rows=64, dtype=1, fmt=1):
+        # 64 rows: quantised in front of the product
         return L.nqx_linear(x, stride, at, at, None, at, rows, 64, 64, dtype, fmt, space, ws_bytes, None)
 
-    need = L.nqx_linear_workspace_bytes(64, 64, 64, 1, 1)
+    need = L.nqx_linear_workspace_bytes(64, 64, 64, 1, 1, 0)
     assert need >= 64 * 64 + 64 * 2
     assert linear(ws_bytes=need - 1) == linear(space=None) == linear(space=at + 8) == 3 and b"workspace" in L.nqx_last_error()
     assert linear(x=at + 2) == linear(stride=60) == linear(dtype=5) == linear(fmt=-1) == 1
-    assert L.nqx_linear_workspace_bytes(64, 64, 33, 1, 1) == 0
+    assert L.nqx_linear_workspace_bytes(64, 64, 33, 1, 1, 0) == 0
+    # a product whose k is split over workgroups has sums to keep
+    split = L.nqx_linear_workspace_bytes(4, 256, 8192, 1, 1, 1)
+    assert split >= 4 * 256 * 4 * 2
+    assert L.nqx_linear_quantized(at, at, at, at, None, at, 4, 256, 8192, 1, 1, at, split - 1, None) == 3
+    assert L.nqx_linear_quantized(at, at, at, at, None, at, 4, 256, 8192, 1, 1, None, split, None) == 3
 
     def norm(x=at, xs=64, delta=at, ds=64, weight=at, total=at, codes=at, scales=at, rows=4, k=64, dtype=1, fmt=1):
         return L.nqx_add_rmsnorm(x, xs, delta, ds, weight, total, codes, scales, rows, k, 1e-6, dtype, fmt, None)
