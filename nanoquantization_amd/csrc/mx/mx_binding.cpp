@@ -3,6 +3,7 @@
 // belongs to the call, so calls on several streams and captured graphs do not share it) and launches on torch's current
 // stream of the tensors' device.  HIP and Meta kernels; inference only (none has a derivative), and no CPU kernel.
 #include <ATen/ATen.h>
+#include <ATen/hip/EmptyTensor.h>
 #include <ATen/hip/impl/HIPGuardImplMasqueradingAsCUDA.h>
 #include <ATen/hip/impl/HIPStreamMasqueradingAsCUDA.h>
 #include <torch/library.h>
@@ -60,15 +61,19 @@ Rows rows_of(const at::Tensor& x) {
     return {t, rows, k, rows > 1 ? t.stride(0) : k};
 }
 
-std::vector<int64_t> with_last(const at::Tensor& x, int64_t last) {
-    std::vector<int64_t> s = x.sizes().vec();
+at::DimVector with_last(const at::Tensor& x, int64_t last) {
+    at::DimVector s(x.sizes());
     s.back() = last;
     return s;
 }
+// An empty tensor beside x: on a HIP device by the allocator's own function, without the dispatcher's round.
+at::Tensor empty_beside(const at::Tensor& x, at::IntArrayRef sizes, at::ScalarType dtype) {
+    if (x.is_cuda()) return at::detail::empty_cuda(sizes, dtype, x.device(), c10::nullopt);
+    return at::empty(sizes, x.options().dtype(dtype));
+}
 Two packed_like(const at::Tensor& x, int format) {
     const int64_t k = x.size(-1);
-    const auto o = x.options().dtype(at::kByte);
-    return {at::empty(with_last(x, format == NQX_FP4 ? k / 2 : k), o), at::empty(with_last(x, k / kBlock), o)};
+    return {empty_beside(x, with_last(x, format == NQX_FP4 ? k / 2 : k), at::kByte), empty_beside(x, with_last(x, k / kBlock), at::kByte)};
 }
 
 // The values a row of codes and scales stands for, and its format, which follows from the two sizes.
@@ -121,7 +126,7 @@ at::Tensor mx_dequantize(const at::Tensor& codes, const at::Tensor& scales, at::
     const int d = dtype_id(dtype);
     check_device(codes, {&scales});
     const DeviceGuard guard(codes.device());
-    at::Tensor y = at::empty(with_last(codes, p.k), codes.options().dtype(dtype));
+    at::Tensor y = empty_beside(codes, with_last(codes, p.k), dtype);
     if (y.numel() == 0) return y;
     const at::Tensor c = dense16(codes), s = scales.contiguous();
     check_status(nqx_dequantize(c.data_ptr<uint8_t>(), s.data_ptr<uint8_t>(), y.data_ptr(), y.numel() / p.k, p.k, d, p.format, stream_of(codes)),
@@ -130,7 +135,7 @@ at::Tensor mx_dequantize(const at::Tensor& codes, const at::Tensor& scales, at::
 }
 at::Tensor mx_dequantize_meta(const at::Tensor& codes, const at::Tensor& scales, at::ScalarType dtype) {
     dtype_id(dtype);
-    return at::empty(with_last(codes, check_packed(codes, scales, "mx_dequantize").k), codes.options().dtype(dtype));
+    return empty_beside(codes, with_last(codes, check_packed(codes, scales, "mx_dequantize").k), dtype);
 }
 
 at::Tensor mx_linear(const at::Tensor& x, const at::Tensor& weight, const at::Tensor& weight_scales, const OptTensor& bias,
@@ -139,13 +144,13 @@ at::Tensor mx_linear(const at::Tensor& x, const at::Tensor& weight, const at::Te
     const int64_t k = last_size(x, "x"), n = check_weight(weight, weight_scales, k);
     check_device(x, {&weight, &weight_scales});
     const DeviceGuard guard(x.device());
-    at::Tensor y = at::empty(with_last(x, n), x.options());
+    at::Tensor y = empty_beside(x, with_last(x, n), x.scalar_type());
     const at::Tensor b = dense_bias(bias, x, n, x.scalar_type());
     if (y.numel() == 0) return y;
     const Rows r = rows_of(x);
     const at::Tensor w = dense16(weight), ws = weight_scales.contiguous();
     const size_t bytes = nqx_linear_workspace_bytes(r.rows, n, k, d, f, 0);
-    const at::Tensor space = bytes ? at::empty({(int64_t)bytes}, w.options()) : at::Tensor();
+    const at::Tensor space = bytes ? empty_beside(w, {(int64_t)bytes}, at::kByte) : at::Tensor();
     check_status(nqx_linear(r.t.data_ptr(), r.stride, w.data_ptr<uint8_t>(), ws.data_ptr<uint8_t>(), b.defined() ? b.data_ptr() : nullptr,
                             y.data_ptr(), r.rows, n, k, d, f, bytes ? space.data_ptr() : nullptr, bytes, stream_of(x)),
                  "nqx_linear");
@@ -155,7 +160,7 @@ at::Tensor mx_linear_meta(const at::Tensor& x, const at::Tensor& weight, const a
                           c10::string_view activations) {
     format_id(activations);
     dtype_id(x.scalar_type());
-    return at::empty(with_last(x, check_weight(weight, weight_scales, last_size(x, "x"))), x.options());
+    return empty_beside(x, with_last(x, check_weight(weight, weight_scales, last_size(x, "x"))), x.scalar_type());
 }
 
 at::Tensor mx_linear_quantized(const at::Tensor& codes, const at::Tensor& scales, const at::Tensor& weight, const at::Tensor& weight_scales,
@@ -165,13 +170,13 @@ at::Tensor mx_linear_quantized(const at::Tensor& codes, const at::Tensor& scales
     const int64_t n = check_weight(weight, weight_scales, p.k);
     check_device(codes, {&scales, &weight, &weight_scales});
     const DeviceGuard guard(codes.device());
-    at::Tensor y = at::empty(with_last(codes, n), codes.options().dtype(dtype));
+    at::Tensor y = empty_beside(codes, with_last(codes, n), dtype);
     const at::Tensor b = dense_bias(bias, codes, n, dtype);
     if (y.numel() == 0) return y;
     const at::Tensor c = dense16(codes), s = scales.contiguous(), w = dense16(weight), ws = weight_scales.contiguous();
     const int64_t rows = y.numel() / n;
     const size_t bytes = nqx_linear_workspace_bytes(rows, n, p.k, d, p.format, 1);
-    const at::Tensor space = bytes ? at::empty({(int64_t)bytes}, w.options()) : at::Tensor();
+    const at::Tensor space = bytes ? empty_beside(w, {(int64_t)bytes}, at::kByte) : at::Tensor();
     check_status(nqx_linear_quantized(c.data_ptr<uint8_t>(), s.data_ptr<uint8_t>(), w.data_ptr<uint8_t>(), ws.data_ptr<uint8_t>(),
                                       b.defined() ? b.data_ptr() : nullptr, y.data_ptr(), rows, n, p.k, d, p.format,
                                       bytes ? space.data_ptr() : nullptr, bytes, stream_of(codes)),
@@ -181,7 +186,7 @@ at::Tensor mx_linear_quantized(const at::Tensor& codes, const at::Tensor& scales
 at::Tensor mx_linear_quantized_meta(const at::Tensor& codes, const at::Tensor& scales, const at::Tensor& weight,
                                     const at::Tensor& weight_scales, const OptTensor&, at::ScalarType dtype) {
     dtype_id(dtype);
-    return at::empty(with_last(codes, check_weight(weight, weight_scales, check_packed(codes, scales, "x").k)), codes.options().dtype(dtype));
+    return empty_beside(codes, with_last(codes, check_weight(weight, weight_scales, check_packed(codes, scales, "x").k)), dtype);
 }
 
 void check_norm(const at::Tensor& x, const at::Tensor& weight) {
@@ -213,7 +218,7 @@ Three mx_add_rmsnorm(const at::Tensor& x, const at::Tensor& delta, const at::Ten
     check_alike(x, delta, "x and delta");
     check_device(x, {&delta, &weight});
     const DeviceGuard guard(x.device());
-    const at::Tensor total = at::empty(x.sizes(), x.options());
+    const at::Tensor total = empty_beside(x, x.sizes(), x.scalar_type());
     Two out = norm(x, delta, weight, eps, f, total);
     return {std::get<0>(out), std::get<1>(out), total};
 }
@@ -222,7 +227,7 @@ Three mx_add_rmsnorm_meta(const at::Tensor& x, const at::Tensor& delta, const at
     check_norm(x, weight);
     check_alike(x, delta, "x and delta");
     Two out = packed_like(x, format_id(format));
-    return {std::get<0>(out), std::get<1>(out), at::empty(x.sizes(), x.options())};
+    return {std::get<0>(out), std::get<1>(out), empty_beside(x, x.sizes(), x.scalar_type())};
 }
 Two mx_rmsnorm(const at::Tensor& x, const at::Tensor& weight, double eps, c10::string_view format) {
     const int f = format_id(format);

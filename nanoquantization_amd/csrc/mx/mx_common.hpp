@@ -3,8 +3,10 @@
 
 #include <hip/hip_runtime.h>
 
+#include <atomic>
 #include <cstddef>
 #include <cstdint>
+#include <tuple>
 
 #include "../../../include/nq_mx_ops.h"
 
@@ -132,7 +134,29 @@ __device__ __forceinline__ void quantize8(const float (&v)[8], uint8_t* codes, u
 
 // ---- host ----------------------------------------------------------------------------------------------------------------
 int refuse(int status, const char* fmt, ...);
-int hip_status(const char* fn);      // of the launch just made
+int hip_status(const char* fn, hipError_t e);
+
+// Launches a kernel; what an earlier call of anybody's has left behind is not taken for this one's error.
+template <typename... P, typename... A>
+static inline hipError_t start(void (*kernel)(P...), dim3 grid, unsigned threads, size_t lds, hipStream_t stream, A... args) {
+    std::tuple<P...> held(args...);
+    return std::apply([&](auto&... a) {
+        void* at[] = {const_cast<void*>(static_cast<const void*>(&a))...};
+        return hipLaunchKernel(reinterpret_cast<const void*>(kernel), grid, dim3(threads), at, lds, stream);
+    }, held);
+}
+// More than 64 KiB of LDS for a kernel, once for each device.
+template <auto KERNEL>
+static inline hipError_t allow_lds(int bytes) {
+    static std::atomic<uint64_t> done{0};
+    int device = 0;
+    if (const hipError_t e = hipGetDevice(&device); e != hipSuccess) return e;
+    const uint64_t bit = 1ull << (device & 63);
+    if (done.load(std::memory_order_relaxed) & bit) return hipSuccess;
+    const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(KERNEL), hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    if (e == hipSuccess) done.fetch_or(bit, std::memory_order_relaxed);
+    return e;
+}
 static inline int64_t cdiv(int64_t a, int64_t b) { return (a + b - 1) / b; }
 static inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 static inline int64_t elem_bytes(int dtype) { return dtype == NQX_F32 ? 4 : 2; }

@@ -17,8 +17,7 @@ int refuse(int status, const char* fmt, ...) {
     return status;
 }
 
-int hip_status(const char* fn) {
-    const hipError_t e = hipGetLastError();
+int hip_status(const char* fn, hipError_t e) {
     return e == hipSuccess ? NQX_OK : refuse(NQX_ERR_HIP, "%s: HIP error %d (%s)", fn, (int)e, hipGetErrorString(e));
 }
 

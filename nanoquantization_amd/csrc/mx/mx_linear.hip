@@ -24,12 +24,19 @@ enum Form { kSkinny, kStream, kTiles128, kTiles256 };
 // Which kernel runs a product.
 Form form_of(int64_t rows, int64_t n, int64_t k) {
     if (k > ((int64_t)1 << 22)) return kSkinny;              // byte offsets in a tile are 32 bits
+    // One launch without a split while that is shorter than a split product and the launch that adds its sums: one row by 4096 x
+    // 12288 7.7 us and 7.1 + 1.7, by 5120 x 25600 18.7 and 12.9 + 1.3; 16 rows, which every 16 weight rows read again, by 2560 x 9728
+    // 14.7 and 8 + 2.
+    if (rows <= 4 ? n * k <= ((int64_t)64 << 20) : rows <= 16 && rows * n * k <= ((int64_t)128 << 20)) return kSkinny;
     if (rows <= 128) return kStream;
     return cdiv(rows, 256) * cdiv(n, 256) >= 192 ? kTiles256 : kTiles128;
 }
-// Whether a linear quantises x in the product's own kernel.
+// Whether a linear quantises x in the product's own kernel: 16 rows, and room in LDS for what a workgroup keeps of them.
 bool raw_of(int64_t rows, int64_t n, int64_t k, int format) {
-    return rows <= 16 && form_of(rows, n, k) == kStream && stream_raw_bytes(rows, n, k, format) <= 48 * 1024;
+    if (rows > 16) return false;
+    const Form form = form_of(rows, n, k);
+    return form == kStream ? stream_raw_bytes(rows, n, k, format) <= 48 * 1024
+                           : form == kSkinny && skinny_raw_bytes(rows, k, format) <= 48 * 1024;
 }
 int product(const Product& p, hipStream_t stream) {
     switch (form_of(p.rows, p.n, p.k)) {
@@ -108,6 +115,6 @@ extern "C" const char* nqx_linear_form(int64_t rows, int64_t n, int64_t k, int d
         case kTiles256: return "mx_tiles_kernel 256 x 256";
         case kTiles128: return "mx_tiles_kernel 128 x 128";
         case kStream: return !quantised && raw_of(rows, n, k, format) ? "mx_stream_kernel on x as it is" : "mx_stream_kernel";
-        default: return "mx_skinny_kernel";
+        default: return !quantised && raw_of(rows, n, k, format) ? "mx_skinny_kernel on x as it is" : "mx_skinny_kernel";
     }
 }

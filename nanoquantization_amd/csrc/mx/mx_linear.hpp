@@ -59,7 +59,8 @@ __device__ __forceinline__ void store_sums(f32x4 v, typename T::elem* y, const t
     }
 }
 
-int skinny_product(const Product& p, hipStream_t stream);
+int skinny_product(const Product& p, hipStream_t stream);       // at most 16 rows of raw x
+int64_t skinny_raw_bytes(int64_t rows, int64_t k, int format);
 int tiles_product(const Product& p, int tile, hipStream_t stream);
 int stream_product(const Product& p, hipStream_t stream);       // at most 128 rows, at most 16 of raw x
 int stream_splits(int64_t rows, int64_t n, int64_t k, int format);

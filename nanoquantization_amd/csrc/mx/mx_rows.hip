@@ -133,13 +133,14 @@ int grid_for(int64_t eights) {
 
 int quantize(const void* x, int64_t x_stride, uint8_t* codes, uint8_t* scales, int64_t rows, int64_t k, int dtype, int format,
              hipStream_t stream) {
+    hipError_t e = hipSuccess;
     by_type(dtype, format, [&](auto t, auto f) {
         using T = decltype(t);
         const int64_t count = rows * (k / kLane);
-        mx_quantize_kernel<T, decltype(f)::value><<<grid_for(count), kThreads, 0, stream>>>(
+        e = start(&mx_quantize_kernel<T, decltype(f)::value>, dim3(grid_for(count)), kThreads, 0, stream, 
             static_cast<const typename T::elem*>(x), x_stride, codes, scales, count, (uint32_t)(k / kLane));
     });
-    return hip_status("nqx_quantize");
+    return hip_status("nqx_quantize", e);
 }
 
 }  // namespace nqx
@@ -166,13 +167,14 @@ extern "C" int nqx_dequantize(const uint8_t* codes, const uint8_t* scales, void*
     if (rows == 0) return NQX_OK;
     if (int s = check_rows("nqx_dequantize", "y", y, k, k, dtype)) return s;
     if (int s = check_out("nqx_dequantize", codes, scales)) return s;
+    hipError_t e = hipSuccess;
     by_type(dtype, format, [&](auto t, auto f) {
         using T = decltype(t);
         const int64_t count = rows * (k / kLane);
-        mx_dequantize_kernel<T, decltype(f)::value><<<grid_for(count), kThreads, 0, static_cast<hipStream_t>(stream)>>>(
+        e = start(&mx_dequantize_kernel<T, decltype(f)::value>, dim3(grid_for(count)), kThreads, 0, static_cast<hipStream_t>(stream), 
             codes, scales, static_cast<typename T::elem*>(y), count);
     });
-    return hip_status("nqx_dequantize");
+    return hip_status("nqx_dequantize", e);
 }
 
 extern "C" int nqx_add_rmsnorm(const void* x, int64_t x_stride, const void* delta, int64_t delta_stride, const void* weight,
@@ -195,12 +197,12 @@ extern "C" int nqx_add_rmsnorm(const void* x, int64_t x_stride, const void* delt
             return refuse(NQX_ERR_ARG, "%s: total can be x or delta only where their rows are k apart", fn);
     }
     if (int s = check_out(fn, codes, scales)) return s;
+    hipError_t e = hipSuccess;
     by_type(dtype, format, [&](auto t, auto f) {
         using T = decltype(t);
         using E = typename T::elem;
         const auto with = [&](auto chunks) {
-            mx_add_rmsnorm_kernel<T, decltype(f)::value, decltype(chunks)::value>
-                <<<(unsigned)rows, kThreads, 0, static_cast<hipStream_t>(stream)>>>(
+            e = start(&mx_add_rmsnorm_kernel<T, decltype(f)::value, decltype(chunks)::value>, dim3((unsigned)rows), kThreads, 0, static_cast<hipStream_t>(stream), 
                     static_cast<const E*>(x), x_stride, static_cast<const E*>(delta), delta_stride, static_cast<const E*>(weight),
                     static_cast<E*>(total), codes, scales, (uint32_t)(k / kLane), eps);
         };
@@ -210,7 +212,7 @@ extern "C" int nqx_add_rmsnorm(const void* x, int64_t x_stride, const void* delt
         else if (chunks <= 4) with(Const<4>());
         else with(Const<8>());
     });
-    return hip_status(fn);
+    return hip_status(fn, e);
 }
 
 extern "C" int nqx_silu_mul(const void* gate, int64_t gate_stride, const void* up, int64_t up_stride, uint8_t* codes,
@@ -221,13 +223,14 @@ extern "C" int nqx_silu_mul(const void* gate, int64_t gate_stride, const void* u
     if (int s = check_rows(fn, "gate", gate, gate_stride, k, dtype)) return s;
     if (int s = check_rows(fn, "up", up, up_stride, k, dtype)) return s;
     if (int s = check_out(fn, codes, scales)) return s;
+    hipError_t e = hipSuccess;
     by_type(dtype, format, [&](auto t, auto f) {
         using T = decltype(t);
         using E = typename T::elem;
         const int64_t count = rows * (k / kLane);
-        mx_silu_mul_kernel<T, decltype(f)::value><<<grid_for(count), kThreads, 0, static_cast<hipStream_t>(stream)>>>(
+        e = start(&mx_silu_mul_kernel<T, decltype(f)::value>, dim3(grid_for(count)), kThreads, 0, static_cast<hipStream_t>(stream), 
             static_cast<const E*>(gate), gate_stride, static_cast<const E*>(up), up_stride, codes, scales, count,
             (uint32_t)(k / kLane));
     });
-    return hip_status(fn);
+    return hip_status(fn, e);
 }

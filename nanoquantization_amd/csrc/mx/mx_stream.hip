@@ -1,7 +1,7 @@
 // The product for up to 128 rows of x, where what counts is to stream the packed weight once: 0.53 bytes a value, and all of x
-// per 128 weight rows.  A workgroup has 128 weight rows, all rows of x and a run of k; its four waves take 32 weight rows each.
-// Operands come to LDS by load-to-LDS in chunks of 256 values of k, whole 128-byte lines of a weight row, two chunks ahead of the
-// one that is multiplied; one barrier a chunk.  Where the weight has too few rows for the chip, k is split over workgroups, whose
+// per workgroup.  A workgroup has 128 weight rows, or 256 where there is more of x to share, all rows of x and a run of k; a wave
+// takes 32 weight rows.  Operands come to LDS by load-to-LDS in chunks of 256 values of k, whole 128-byte lines of a weight row,
+// two chunks ahead of the one that is multiplied, or one; one barrier a chunk.  Where the weight has too few rows for the chip, k is split over workgroups, whose
 // sums go to memory in fp32 and are added, in the order of the splits, by a second kernel.
 //
 // With RAW x comes as it is and every workgroup quantises its run of it into LDS first, while its first chunks are on their way:
@@ -11,18 +11,24 @@
 namespace nqx {
 namespace {
 
-constexpr int kRows = 128, kThreads = 256, kBufs = 3;
+// By sixteens of rows of x: weight rows of a workgroup, buffers, and the workgroups that fit a CU's LDS.  64 rows by 5120 x 25600 with
+// 128 weight rows and three buffers for any x: 26 us, 128 rows 43.
+constexpr int weight_rows(int mt) { return mt >= 4 ? 256 : 128; }
+constexpr int buffers(int mt) { return mt == 1 ? 3 : 2; }
+constexpr int per_cu(int mt) { return mt <= 2 ? 2 : 1; }
+int sixteens(int64_t rows) { return rows <= 16 ? 1 : rows <= 32 ? 2 : rows <= 64 ? 4 : 8; }
 
 template <int FORMAT, int MT, bool RAW>
 struct Stream {
+    static constexpr int kRows = weight_rows(MT), kWaves = kRows / 32, kThreads = 64 * kWaves, kBufs = buffers(MT);
     static constexpr int kHalves = FORMAT == NQX_FP4 ? 1 : 2;          // 128-byte parts of a row of x in a chunk
     static constexpr int kW = kRows * 128, kXHalf = 16 * MT * 128, kX = RAW ? 0 : kHalves * kXHalf, kBuf = kW + kX;
-    static constexpr int kWLoads = kRows / 32, kXAll = RAW ? 0 : 2 * MT * kHalves, kXLoads = (kXAll + 3) / 4;    // of a wave, 1 KiB each
+    static constexpr int kWLoads = 4, kXAll = RAW ? 0 : 2 * MT * kHalves, kXLoads = (kXAll + kWaves - 1) / kWaves;    // of a wave, 1 KiB each
     static constexpr int kLoads = kWLoads + kXLoads;
     static constexpr int kNone = kBufs * kBuf;                         // where a wave without a piece of x lets its request go
-    static constexpr int kScales = kNone + (kXAll % 4 ? 1024 : 0), kSlot = (kRows + (RAW ? 0 : 16 * MT)) * 32;
+    static constexpr int kScales = kNone + (kXAll % kWaves ? 1024 : 0), kSlot = (kRows + (RAW ? 0 : 16 * MT)) * 32;
     static constexpr int kFixed = kScales + 2 * kSlot;
-    static_assert(kFixed <= 160 * 1024, "");
+    static_assert(kFixed * per_cu(MT) <= 160 * 1024 && kLoads < 16, "");
 };
 // RAW: bytes of `rows` quantised rows of `chunks` chunks in LDS, codes and scales.
 __host__ __device__ constexpr int resident_bytes(int format, int rows, int chunks) {
@@ -30,13 +36,14 @@ __host__ __device__ constexpr int resident_bytes(int format, int rows, int chunk
 }
 
 template <typename T, int FORMAT, int MT, bool RAW>
-__global__ __launch_bounds__(kThreads) void mx_stream_kernel(const void* __restrict__ x, int64_t x_stride, const uint8_t* __restrict__ xs,
+__global__ __launch_bounds__(2 * weight_rows(MT)) void mx_stream_kernel(const void* __restrict__ x, int64_t x_stride, const uint8_t* __restrict__ xs,
                                                              const uint8_t* __restrict__ w, const uint8_t* __restrict__ ws,
                                                              const typename T::elem* __restrict__ bias, typename T::elem* __restrict__ y,
                                                              float* __restrict__ sums, int rows, int N, int blocks, int words, int tiles,
                                                              int splits) {
     using G = Stream<FORMAT, MT, RAW>;
     constexpr bool kFour = FORMAT == NQX_FP4;
+    constexpr int kRows = G::kRows, kWaves = G::kWaves, kThreads = G::kThreads, kBufs = G::kBufs;
     extern __shared__ __attribute__((aligned(16))) unsigned char s_mem[];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lo = lane & 15, hi = lane >> 4;
     const int split = blockIdx.x / tiles, n0 = (blockIdx.x - split * tiles) * kRows;
@@ -68,12 +75,12 @@ __global__ __launch_bounds__(kThreads) void mx_stream_kernel(const void* __restr
         const int at = (c % kBufs) * G::kBuf, f = partial ? whole : c - first;
 #pragma unroll
         for (int q = 0; q < G::kWLoads; ++q) {
-            const int i = wave + 4 * q, r = 8 * i + (lane >> 3), piece = swizzle(r, lane & 7);
+            const int i = wave + kWaves * q, r = 8 * i + (lane >> 3), piece = swizzle(r, lane & 7);
             bring(buffer(wb, there ? n_rows * w_pitch : 0), partial && piece >= part ? kNowhere : r * w_pitch + piece * 16, at + i * 1024, f * 128);
         }
 #pragma unroll
         for (int q = 0; q < G::kXLoads; ++q) {
-            const int i = wave + 4 * q, h = i / (2 * MT), r = 8 * (i % (2 * MT)) + (lane >> 3), piece = swizzle(r, lane & 7);
+            const int i = wave + kWaves * q, h = i / (2 * MT), r = 8 * (i % (2 * MT)) + (lane >> 3), piece = swizzle(r, lane & 7);
             const bool mine = i < G::kXAll, none = partial && (kFour ? piece >= part : 8 * h + piece >= 2 * part);
             bring(buffer(xb, there && mine ? rows * x_pitch : 0), none ? kNowhere : r * x_pitch + piece * 16,
                   mine ? at + G::kW + i * 1024 : G::kNone, f * 128 * G::kHalves + h * 128);
@@ -90,11 +97,11 @@ __global__ __launch_bounds__(kThreads) void mx_stream_kernel(const void* __restr
         if (g >= g1) return;
         const int at = start_of(g), slot = G::kScales + (g & 1) * G::kSlot;
         if (words) {
-            for (int i = wave; i < kRows / 32; i += 4)
+            for (int i = wave; i < kRows / 32; i += kWaves)
                 bring(buffer(wsb, n_rows * blocks), (32 * i + (lane >> 1)) * blocks + (lane & 1) * 16, slot + i * 1024, at);
             if constexpr (!RAW) {
                 // 16 rows of x are half a request's: the other lanes' are past the end, and past the slot's rows
-                for (int i = wave; i < (16 * MT + 31) / 32; i += 4) {
+                for (int i = wave; i < (16 * MT + 31) / 32; i += kWaves) {
                     const int r = 32 * i + (lane >> 1);
                     if (16 * MT % 32 == 0 || r < 16 * MT)
                         bring(buffer(xs, rows * blocks), r * blocks + (lane & 1) * 16, slot + kRows * 32 + i * 1024, at);
@@ -133,7 +140,7 @@ __global__ __launch_bounds__(kThreads) void mx_stream_kernel(const void* __restr
 
     ask_scales(g0);
     load(c0);
-    load(c0 + 1);
+    if (kBufs == 3) load(c0 + 1);
     const int chunks = c1 - c0, r_bytes = chunks * (kFour ? 128 : 256);      // RAW: of a row's codes in LDS; the scales behind all of them
     unsigned char* s_x = s_mem + G::kFixed;
     unsigned char* s_xs = s_x + rows * r_bytes;
@@ -163,15 +170,15 @@ __global__ __launch_bounds__(kThreads) void mx_stream_kernel(const void* __restr
     const int w_row = wave * 32 + lo, x_own = lo < rows ? lo : rows - 1;
 #pragma unroll 1
     for (int c = c0; c < c1; ++c) {
-        // chunk c has landed, c + 1 may be on its way; nobody needs the buffer of c - 1 any more
-        __builtin_amdgcn_s_waitcnt(0x0070 | G::kLoads);      // vmcnt(kLoads), lgkmcnt(0)
+        // chunk c has landed, of three buffers c + 1 may be on its way; nobody needs the buffer of c - 1 any more
+        __builtin_amdgcn_s_waitcnt(0x0070 | (kBufs == 3 ? G::kLoads : 0));      // vmcnt(n), lgkmcnt(0)
         __builtin_amdgcn_sched_barrier(0);
         __builtin_amdgcn_s_barrier();
         __builtin_amdgcn_sched_barrier(0);
         const int g = c < first ? 0 : first + ((c - first) >> 2);
         const bool begins = c == chunk_of(g);
         if (begins) ask_scales(g + 1);
-        load(c + 2);
+        load(c + kBufs - 1);
         const int at = (c % kBufs) * G::kBuf;
         // where the chunk's scales are in the group's bytes; of the chunk that is not whole a block that is none has zeros for codes
         // and the scale of the last block, which is no NaN unless the row's sum is
@@ -244,24 +251,20 @@ template <typename T, int FORMAT, int MT, bool RAW>
 hipError_t launch(const Product& p, hipStream_t stream) {
     using G = Stream<FORMAT, MT, RAW>;
     using E = typename T::elem;
-    const int blocks = (int)(p.k / kBlock), tiles = (int)cdiv(p.n, kRows), splits = stream_splits(p.rows, p.n, p.k, p.format);
+    const int blocks = (int)(p.k / kBlock), tiles = (int)cdiv(p.n, G::kRows), splits = stream_splits(p.rows, p.n, p.k, p.format);
     const int chunks = (blocks & 7 ? 1 : 0) + (blocks >> 3);
     const int lds = G::kFixed + (RAW ? resident_bytes(FORMAT, (int)p.rows, stream_chunks(chunks, blocks, splits)) : 0);
-    if (lds > 64 * 1024) {
-        const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(&mx_stream_kernel<T, FORMAT, MT, RAW>),
-                                                 hipFuncAttributeMaxDynamicSharedMemorySize, 160 * 1024);
-        if (e != hipSuccess) return e;
-    }
+    if (lds > 64 * 1024)
+        if (const hipError_t e = allow_lds<&mx_stream_kernel<T, FORMAT, MT, RAW>>(160 * 1024); e != hipSuccess) return e;
     const int words = blocks % 4 == 0 && blocks >= 32 && ((reinterpret_cast<uintptr_t>(p.ws) | reinterpret_cast<uintptr_t>(p.xs)) & 3) == 0;
     const E *bias = static_cast<const E*>(p.bias);
     E* y = static_cast<E*>(p.y);
-    mx_stream_kernel<T, FORMAT, MT, RAW><<<tiles * splits, kThreads, lds, stream>>>(
-        RAW ? p.raw : p.x, p.raw_stride, p.xs, p.w, p.ws, bias, y, p.sums, (int)p.rows, (int)p.n, blocks, words, tiles, splits);
-    if (splits > 1) {
-        const int pitch = tiles * kRows;
-        mx_add_splits_kernel<T><<<(unsigned)cdiv(p.rows * pitch, 1024), 256, 0, stream>>>(p.sums, bias, y, (int)p.rows, (int)p.n, pitch, splits);
-    }
-    return hipGetLastError();
+    const hipError_t e = start(&mx_stream_kernel<T, FORMAT, MT, RAW>, dim3(tiles * splits), G::kThreads, lds, stream, RAW ? p.raw : p.x,
+                               p.raw_stride, p.xs, p.w, p.ws, bias, y, p.sums, (int)p.rows, (int)p.n, blocks, words, tiles, splits);
+    if (e != hipSuccess || splits == 1) return e;
+    const int pitch = tiles * G::kRows;
+    return start(&mx_add_splits_kernel<T>, dim3((unsigned)cdiv(p.rows * pitch, 1024)), 256, 0, stream, p.sums, bias, y, (int)p.rows, (int)p.n,
+                 pitch, splits);
 }
 
 }  // namespace
@@ -272,19 +275,19 @@ int stream_product(const Product& p, hipStream_t stream) {
         using T = decltype(t);
         constexpr int F = decltype(f)::value;
         if (p.raw) e = launch<T, F, 1, true>(p, stream);
-        else if (p.rows <= 16) e = launch<T, F, 1, false>(p, stream);
-        else if (p.rows <= 32) e = launch<T, F, 2, false>(p, stream);
-        else if (p.rows <= 64) e = launch<T, F, 4, false>(p, stream);
+        else if (sixteens(p.rows) == 1) e = launch<T, F, 1, false>(p, stream);
+        else if (sixteens(p.rows) == 2) e = launch<T, F, 2, false>(p, stream);
+        else if (sixteens(p.rows) == 4) e = launch<T, F, 4, false>(p, stream);
         else e = launch<T, F, 8, false>(p, stream);
     });
-    return e == hipSuccess ? NQX_OK : refuse(NQX_ERR_HIP, "mx_stream_kernel: HIP error %d (%s)", (int)e, hipGetErrorString(e));
+    return hip_status("mx_stream_kernel", e);
 }
 
-// Workgroups for the chip twice over, each with a group of chunks at least.
+// As many splits as fill the chip with workgroups that are resident at once, of a group of chunks each at least.
 int stream_splits(int64_t rows, int64_t n, int64_t k, int) {
-    const int64_t tiles = cdiv(n, kRows), blocks = k / kBlock, groups = (blocks & 7 ? 1 : 0) + ((blocks >> 3) + 3) / 4;
-    const int64_t want = rows <= 64 ? 512 : 256;
-    int64_t s = want / tiles;
+    const int mt = sixteens(rows);
+    const int64_t tiles = cdiv(n, weight_rows(mt)), blocks = k / kBlock, groups = (blocks & 7 ? 1 : 0) + ((blocks >> 3) + 3) / 4;
+    int64_t s = 256 * per_cu(mt) / tiles;
     if (s > groups) s = groups;
     if (s > 16) s = 16;
     return s < 1 ? 1 : (int)s;
@@ -297,7 +300,8 @@ int stream_chunks(int chunks, int blocks, int splits) {
 }
 size_t stream_sums_bytes(int64_t rows, int64_t n, int64_t k, int format) {
     const int64_t s = stream_splits(rows, n, k, format);
-    return s > 1 ? (size_t)(s * rows * cdiv(n, kRows) * kRows * 4) : 0;
+    const int64_t tile = weight_rows(sixteens(rows));
+    return s > 1 ? (size_t)(s * rows * cdiv(n, tile) * tile * 4) : 0;
 }
 int stream_raw_bytes(int64_t rows, int64_t n, int64_t k, int format) {
     const int blocks = (int)(k / kBlock), chunks = (blocks & 7 ? 1 : 0) + (blocks >> 3);

@@ -389,14 +389,11 @@ hipError_t launch(const Product& p, hipStream_t stream) {
     using G = Tiles<FORMAT, S>;
     using E = typename T::elem;
     const int x_tiles = (int)cdiv(p.rows, S), w_tiles = (int)cdiv(p.n, S);
-    const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(&mx_tiles_kernel<T, FORMAT, S, BIAS>),
-                                             hipFuncAttributeMaxDynamicSharedMemorySize, G::kLds);
-    if (e != hipSuccess) return e;
+    if (const hipError_t e = allow_lds<&mx_tiles_kernel<T, FORMAT, S, BIAS>>(G::kLds); e != hipSuccess) return e;
     const unsigned grid = (unsigned)(cdiv((int64_t)x_tiles * w_tiles, 8) * 8);
-    mx_tiles_kernel<T, FORMAT, S, BIAS><<<grid, G::kThreads, G::kLds, stream>>>(
-        p.x, p.xs, p.w, p.ws, static_cast<const E*>(p.bias), static_cast<E*>(p.y), (int)p.rows, (int)p.n, (int)(p.k / kBlock),
-        p.k / kBlock % 4 == 0 && ((reinterpret_cast<uintptr_t>(p.ws) | reinterpret_cast<uintptr_t>(p.xs)) & 3) == 0, x_tiles, w_tiles);
-    return hipGetLastError();
+    const int words = p.k / kBlock % 4 == 0 && ((reinterpret_cast<uintptr_t>(p.ws) | reinterpret_cast<uintptr_t>(p.xs)) & 3) == 0;
+    return start(&mx_tiles_kernel<T, FORMAT, S, BIAS>, dim3(grid), G::kThreads, G::kLds, stream, p.x, p.xs, p.w, p.ws,
+                 static_cast<const E*>(p.bias), static_cast<E*>(p.y), (int)p.rows, (int)p.n, (int)(p.k / kBlock), words, x_tiles, w_tiles);
 }
 
 }  // namespace
@@ -409,7 +406,7 @@ int tiles_product(const Product& p, int tile, hipStream_t stream) {
         if (p.bias) e = tile == 256 ? launch<T, F, 256, true>(p, stream) : launch<T, F, 128, true>(p, stream);
         else e = tile == 256 ? launch<T, F, 256, false>(p, stream) : launch<T, F, 128, false>(p, stream);
     });
-    return e == hipSuccess ? NQX_OK : refuse(NQX_ERR_HIP, "mx_tiles_kernel: HIP error %d (%s)", (int)e, hipGetErrorString(e));
+    return hip_status("mx_tiles_kernel", e);
 }
 
 }  // namespace nqx

@@ -22,53 +22,70 @@ MX_BLOCK = 32
 MX_FORMATS = ("mxfp4", "mxfp8")
 
 
-def _on_device(t: torch.Tensor) -> None:
-    if t.device.type != "cuda":
-        raise _lib.AwqHipError("MX kernels run on a HIP device only (tensor is on %s); there is no CPU fallback" % t.device)
+class _Operators:
+    """torch.ops.nanoquantization_amd.mx_*, looked up once."""
+
+    def __getattr__(self, name: str):
+        op = getattr(_lib.mx_ops(), name).default
+        setattr(self, name, op)
+        return op
+
+
+_ops = _Operators()
+
+
+def _elsewhere(t: torch.Tensor):
+    return _lib.AwqHipError("MX kernels run on a HIP device only (tensor is on %s); there is no CPU fallback" % t.device)
 
 
 def mx_quantize(x: torch.Tensor, format: str = "mxfp4") -> tuple[torch.Tensor, torch.Tensor]:
     """(codes, scales) of x [..., k], float16, bfloat16 or float32."""
-    _on_device(x)
-    return _lib.mx_ops().mx_quantize(x, format)
+    if not x.is_cuda:
+        raise _elsewhere(x)
+    return _ops.mx_quantize(x, format)
 
 
 def mx_dequantize(codes: torch.Tensor, scales: torch.Tensor, dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
     """The values [..., k] that codes and scales stand for, rounded once to `dtype`; the format follows from the sizes."""
-    _on_device(codes)
-    return _lib.mx_ops().mx_dequantize(codes, scales, dtype)
+    if not codes.is_cuda:
+        raise _elsewhere(codes)
+    return _ops.mx_dequantize(codes, scales, dtype)
 
 
 def mx_linear(x: torch.Tensor, weight: torch.Tensor, weight_scales: torch.Tensor, bias: Optional[torch.Tensor] = None,
               activations: str = "mxfp8") -> torch.Tensor:
     """x [..., k] quantised to `activations`, times weight^T, plus bias: [..., n] in x's dtype.  Sums in fp32, one rounding
     behind the bias."""
-    _on_device(x)
-    return _lib.mx_ops().mx_linear(x, weight, weight_scales, bias, activations)
+    if not x.is_cuda:
+        raise _elsewhere(x)
+    return _ops.mx_linear(x, weight, weight_scales, bias, activations)
 
 
 def mx_linear_quantized(codes: torch.Tensor, scales: torch.Tensor, weight: torch.Tensor, weight_scales: torch.Tensor,
                         bias: Optional[torch.Tensor] = None, dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
     """The same product for activations that are quantised already (by mx_quantize, mx_add_rmsnorm or mx_silu_mul)."""
-    _on_device(codes)
-    return _lib.mx_ops().mx_linear_quantized(codes, scales, weight, weight_scales, bias, dtype)
+    if not codes.is_cuda:
+        raise _elsewhere(codes)
+    return _ops.mx_linear_quantized(codes, scales, weight, weight_scales, bias, dtype)
 
 
 def mx_add_rmsnorm(x: torch.Tensor, delta: Optional[torch.Tensor], weight: torch.Tensor, eps: float = 1e-6,
                    format: str = "mxfp8") -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
     """(codes, scales, total): total = x + delta in x's dtype, and the quantised RMSNorm of it times `weight`, computed in fp32
     from the rounded sum.  Without a delta total is x itself.  At most 16384 values a row."""
-    _on_device(x)
+    if not x.is_cuda:
+        raise _elsewhere(x)
     if delta is None:
-        codes, scales = _lib.mx_ops().mx_rmsnorm(x, weight, eps, format)
+        codes, scales = _ops.mx_rmsnorm(x, weight, eps, format)
         return codes, scales, x
-    return _lib.mx_ops().mx_add_rmsnorm(x, delta, weight, eps, format)
+    return _ops.mx_add_rmsnorm(x, delta, weight, eps, format)
 
 
 def mx_silu_mul(gate: torch.Tensor, up: torch.Tensor, format: str = "mxfp8") -> tuple[torch.Tensor, torch.Tensor]:
     """(codes, scales) of SiLU(gate) * up, computed in fp32; the halves of one tensor [..., 2 k] are read in place."""
-    _on_device(gate)
-    return _lib.mx_ops().mx_silu_mul(gate, up, format)
+    if not gate.is_cuda:
+        raise _elsewhere(gate)
+    return _ops.mx_silu_mul(gate, up, format)
 
 
 class MXLinear(nn.Module):

@@ -73,10 +73,10 @@ def test_c_abi_refuses_before_it_launches():
     assert linear(x=at + 2) == linear(stride=60) == linear(dtype=5) == linear(fmt=-1) == 1
     assert L.nqx_linear_workspace_bytes(64, 64, 33, 1, 1, 0) == 0
     # a product whose k is split over workgroups has sums to keep
-    split = L.nqx_linear_workspace_bytes(4, 256, 8192, 1, 1, 1)
-    assert split >= 4 * 256 * 4 * 2
-    assert L.nqx_linear_quantized(at, at, at, at, None, at, 4, 256, 8192, 1, 1, at, split - 1, None) == 3
-    assert L.nqx_linear_quantized(at, at, at, at, None, at, 4, 256, 8192, 1, 1, None, split, None) == 3
+    split = L.nqx_linear_workspace_bytes(20, 256, 8192, 1, 1, 1)
+    assert split >= 20 * 256 * 4 * 2
+    assert L.nqx_linear_quantized(at, at, at, at, None, at, 20, 256, 8192, 1, 1, at, split - 1, None) == 3
+    assert L.nqx_linear_quantized(at, at, at, at, None, at, 20, 256, 8192, 1, 1, None, split, None) == 3
 
     def norm(x=at, xs=64, delta=at, ds=64, weight=at, total=at, codes=at, scales=at, rows=4, k=64, dtype=1, fmt=1):
         return L.nqx_add_rmsnorm(x, xs, delta, ds, weight, total, codes, scales, rows, k, 1e-6, dtype, fmt, None)
