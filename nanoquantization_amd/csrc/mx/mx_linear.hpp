@@ -22,12 +22,12 @@ struct Product {
 
 // One matrix instruction: 16 weight rows x 16 rows of x over 128 values (four blocks).  Lane l has row l % 16 and, with
 // g = l / 16, block g in e2m1 (16 bytes); in e4m3 the 16 bytes of values 16 g .. and those of 64 + 16 g ...  Its scale byte
-// is that of block g for either type.  The result: column l % 16, weight rows 4 g .. 4 g + 3.
-template <int FORMAT>
+// is that of block g for either type, byte BYTE of the word.  The result: column l % 16, weight rows 4 g .. 4 g + 3.
+template <int FORMAT, int BYTE = 0>
 __device__ __forceinline__ f32x4 mfma(u32x4 w, u32x4 x0, u32x4 x1, f32x4 c, uint32_t w_scale, uint32_t x_scale) {
     const i32x8 a = {(int)w[0], (int)w[1], (int)w[2], (int)w[3], 0, 0, 0, 0};
     const i32x8 b = {(int)x0[0], (int)x0[1], (int)x0[2], (int)x0[3], (int)x1[0], (int)x1[1], (int)x1[2], (int)x1[3]};
-    return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, b, c, 4, FORMAT == NQX_FP4 ? 4 : 0, 0, (int)w_scale, 0, (int)x_scale);
+    return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, b, c, 4, FORMAT == NQX_FP4 ? 4 : 0, BYTE, (int)w_scale, BYTE, (int)x_scale);
 }
 
 // e2m1 with e2m1: 32 weight rows x 32 rows of x over 64 values.  Lane l has row l % 32 and one block; with h = l / 32 the result is
@@ -64,7 +64,6 @@ int64_t skinny_raw_bytes(int64_t rows, int64_t k, int format);
 int tiles_product(const Product& p, int tile, hipStream_t stream);
 int stream_product(const Product& p, hipStream_t stream);       // at most 128 rows, at most 16 of raw x
 int stream_splits(int64_t rows, int64_t n, int64_t k, int format);
-int stream_chunks(int chunks, int blocks, int splits);
 size_t stream_sums_bytes(int64_t rows, int64_t n, int64_t k, int format);
 int stream_raw_bytes(int64_t rows, int64_t n, int64_t k, int format);
 
