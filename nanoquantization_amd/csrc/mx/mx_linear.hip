@@ -55,7 +55,7 @@ struct Space {
 Space space_of(int64_t rows, int64_t n, int64_t k, int format, bool quantised) {
     Space s = {0, 0, 0};
     if (rows == 0 || n == 0) return s;
-    if (form_of(rows, n, k) == kStream) s.sums = stream_sums_bytes(rows, n, k, format);
+    if (form_of(rows, n, k) == kStream) s.sums = stream_sums_bytes(rows, n, k);
     if (!quantised && !raw_of(rows, n, k, format)) s.codes = (size_t)(rows * code_bytes(k, format)), s.scales = (size_t)(rows * (k / kBlock));
     return s;
 }

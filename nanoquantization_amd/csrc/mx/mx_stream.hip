@@ -12,10 +12,12 @@
 namespace nqx {
 namespace {
 
-// By sixteens of rows of x: weight rows of a workgroup, chunks whose scales come at a time, and the workgroups that fit a CU's LDS.
-constexpr int weight_rows(int mt) { return mt == 4 ? 256 : 128; }
+// By sixteens of rows of x: chunks whose scales come at a time, workgroups that fit a CU's LDS, and how many fours of waves a
+// workgroup has: of two, one has a chunk's first instruction along k and one the second, so that a SIMD has something else to do
+// while a wave waits for LDS.
 constexpr int group_chunks(int mt) { return mt >= 4 ? 2 : 4; }
 constexpr int per_cu(int mt) { return mt == 1 ? 2 : 1; }
+constexpr int fours(int mt) { return mt == 1 ? 1 : 2; }
 // The most chunks that one of `splits` runs has.
 int most_chunks(int chunks, int blocks, int splits, int group) {
     const int first = blocks & 7 ? 1 : 0, whole = chunks - first, groups = first + (whole + group - 1) / group;
@@ -23,17 +25,34 @@ int most_chunks(int chunks, int blocks, int splits, int group) {
     return most < chunks ? most : chunks;
 }
 int sixteens(int64_t rows) { return rows <= 16 ? 1 : rows <= 32 ? 2 : rows <= 64 ? 4 : 8; }
+// Weight rows of a workgroup, and splits of k: as many as fill the chip with workgroups that are resident at once, of a group of
+// chunks each at least.  With 33 to 64 rows of x 256 weight rows share them, unless 128 do without a split, whose sums would cost
+// another launch.
+struct Plan {
+    int weight_rows, splits;
+};
+Plan plan_of(int64_t rows, int64_t n, int64_t k) {
+    const int mt = sixteens(rows), per = group_chunks(mt);
+    const int64_t blocks = k / kBlock, groups = (blocks & 7 ? 1 : 0) + ((blocks >> 3) + per - 1) / per, most = 256 * per_cu(mt);
+    const int wide = mt == 4 && (cdiv(n, 256) >= 160 || cdiv(n, 128) < 160) ? 256 : 128;
+    int64_t s = cdiv(n, wide) >= 160 ? 1 : most / cdiv(n, wide);
+    if (s > groups) s = groups;
+    if (s > 16) s = 16;
+    return {wide, s < 1 ? 1 : (int)s};
+}
 
-template <int FORMAT, int MT, bool RAW>
+template <int FORMAT, int MT, int TW, bool RAW>
 struct Stream {
-    static constexpr int kRows = weight_rows(MT), kWaves = 4, kThreads = 256, kWT = kRows / 64, kBufs = 3, kGroup = group_chunks(MT), kBytes = 8 * kGroup;     // kBytes: a row's scales of a group
+    static constexpr int kRows = TW, kFours = fours(MT), kWaves = 4 * kFours, kThreads = 64 * kWaves, kWT = kRows / 64, kBufs = 3, kGroup = group_chunks(MT), kBytes = 8 * kGroup;     // kBytes: a row's scales of a group
     static constexpr int kHalves = FORMAT == NQX_FP4 ? 1 : 2;          // 128-byte parts of a row of x in a chunk
     static constexpr int kW = kRows * 128, kXHalf = 16 * MT * 128, kX = RAW ? 0 : kHalves * kXHalf, kXAt = kBufs * kW;      // [weight | x]
-    static constexpr int kWLoads = kRows / 32, kXAll = RAW ? 0 : 2 * MT * kHalves, kXLoads = (kXAll + kWaves - 1) / kWaves;    // of a wave, 1 KiB each
+    static constexpr int kWLoads = kRows / 8 / kWaves, kXAll = RAW ? 0 : 2 * MT * kHalves, kXLoads = (kXAll + kWaves - 1) / kWaves;    // of a wave, 1 KiB each
     static constexpr int kLoads = kWLoads + kXLoads;
     static constexpr int kNone = kXAt + kBufs * kX;                         // where a wave without a piece of x lets its request go
     static constexpr int kScales = kNone + (kXAll % kWaves ? 1024 : 0), kSlot = (kRows + (RAW ? 0 : 16 * MT)) * kBytes;
     static constexpr int kFixed = kScales + 2 * kSlot;
+    static constexpr int kMeet = kFours == 2 ? 4 * kWT * MT * 1024 : 0;      // bytes of LDS where the two fours' sums meet, in the buffers' place
+    static_assert(kMeet <= kNone, "");
     static_assert(kFixed * per_cu(MT) <= 160 * 1024 , "");
 };
 // RAW: bytes of `rows` quantised rows of `chunks` chunks in LDS, codes and scales.
@@ -41,15 +60,15 @@ __host__ __device__ constexpr int resident_bytes(int format, int rows, int chunk
     return rows * chunks * ((format == NQX_FP4 ? 128 : 256) + 8);
 }
 
-template <typename T, int FORMAT, int MT, bool RAW>
-__global__ __launch_bounds__(256) void mx_stream_kernel(const void* __restrict__ x, int64_t x_stride, const uint8_t* __restrict__ xs,
+template <typename T, int FORMAT, int MT, int TW, bool RAW>
+__global__ __launch_bounds__(256 * fours(MT)) void mx_stream_kernel(const void* __restrict__ x, int64_t x_stride, const uint8_t* __restrict__ xs,
                                                         const uint8_t* __restrict__ w, const uint8_t* __restrict__ ws,
                                                         const typename T::elem* __restrict__ bias, typename T::elem* __restrict__ y,
                                                         float* __restrict__ sums, int rows, int N, int blocks, int words, int groups_each,
                                                         int groups_more) {
-    using G = Stream<FORMAT, MT, RAW>;
+    using G = Stream<FORMAT, MT, TW, RAW>;
     constexpr bool kFour = FORMAT == NQX_FP4;
-    constexpr int kRows = G::kRows, kThreads = G::kThreads, kWT = G::kWT, kGroup = G::kGroup, kBytes = G::kBytes;
+    constexpr int kRows = G::kRows, kWaves = G::kWaves, kThreads = G::kThreads, kWT = G::kWT, kGroup = G::kGroup, kBytes = G::kBytes;
     extern __shared__ __attribute__((aligned(16))) unsigned char s_mem[];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lo = lane & 15, hi = lane >> 4;
     const int split = blockIdx.y, n0 = blockIdx.x * kRows;
@@ -80,10 +99,10 @@ __global__ __launch_bounds__(256) void mx_stream_kernel(const void* __restrict__
     bool x_mine[G::kXLoads ? G::kXLoads : 1];
     const int piece = swizzle(8 * wave + (lane >> 3), lane & 7);            // of all a lane's loads: their rows are 32 apart
 #pragma unroll
-    for (int q = 0; q < G::kWLoads; ++q) vw[q] = (8 * (wave + 4 * q) + (lane >> 3)) * w_pitch + piece * 16;
+    for (int q = 0; q < G::kWLoads; ++q) vw[q] = (8 * (wave + kWaves * q) + (lane >> 3)) * w_pitch + piece * 16;
 #pragma unroll
     for (int q = 0; q < G::kXLoads; ++q) {
-        const int i = wave + 4 * q, r = 8 * (i % (2 * MT)) + (lane >> 3);
+        const int i = wave + kWaves * q, r = 8 * (i % (2 * MT)) + (lane >> 3);
         x_mine[q] = i < G::kXAll, x_half[q] = i / (2 * MT), x_to[q] = i * 1024;
         vx[q] = x_mine[q] ? r * x_pitch + swizzle(r, lane & 7) * 16 + x_half[q] * 128 : kNowhere;
     }
@@ -95,10 +114,10 @@ __global__ __launch_bounds__(256) void mx_stream_kernel(const void* __restrict__
         const auto bw = buffer(wb, there ? n_rows * w_pitch : 0), bx = buffer(xb, there ? rows * x_pitch : 0);
 #pragma unroll
         for (int q = 0; q < G::kWLoads; ++q)
-            bring(bw, PARTIAL && partial && piece >= part ? kNowhere : vw[q], ring * G::kW + (wave + 4 * q) * 1024, f * 128);
+            bring(bw, PARTIAL && partial && piece >= part ? kNowhere : vw[q], ring * G::kW + (wave + kWaves * q) * 1024, f * 128);
 #pragma unroll
         for (int q = 0; q < G::kXLoads; ++q) {
-            const int r = 8 * ((wave + 4 * q) % (2 * MT)) + (lane >> 3), p = swizzle(r, lane & 7);
+            const int r = 8 * ((wave + kWaves * q) % (2 * MT)) + (lane >> 3), p = swizzle(r, lane & 7);
             const bool none = PARTIAL && partial && (kFour ? p >= part : 8 * x_half[q] + p >= 2 * part);
             bring(bx, none ? kNowhere : vx[q], x_mine[q] ? G::kXAt + ring * G::kX + x_to[q] : G::kNone, f * 128 * G::kHalves);
         }
@@ -116,18 +135,18 @@ __global__ __launch_bounds__(256) void mx_stream_kernel(const void* __restrict__
         const int at = start_of(g), slot = G::kScales + (g & 1) * G::kSlot;
         if (words) {
 #pragma unroll
-            for (int i = 0; i < (kRows * kLanes + 255) / 256; ++i) {
-                const int e = 256 * i + threadIdx.x;
-                if (kRows * kLanes % 256 == 0 || 256 * i + 64 * wave < kRows * kLanes)
-                    bring(buffer(wsb, n_rows * blocks), e / kLanes * blocks + e % kLanes * 16, slot + i * 4096 + wave * 1024, at);
+            for (int i = 0; i < (kRows * kLanes + kThreads - 1) / kThreads; ++i) {
+                const int e = kThreads * i + threadIdx.x;
+                if (kRows * kLanes % kThreads == 0 || kThreads * i + 64 * wave < kRows * kLanes)
+                    bring(buffer(wsb, n_rows * blocks), e / kLanes * blocks + e % kLanes * 16, slot + (kWaves * i + wave) * 1024, at);
             }
             if constexpr (!RAW) {
                 // 16 rows of x are less than a request's: the other lanes' are past the slot
 #pragma unroll
-                for (int i = 0; i < (16 * MT * kLanes + 255) / 256; ++i) {
-                    const int e = 256 * i + threadIdx.x;
+                for (int i = 0; i < (16 * MT * kLanes + kThreads - 1) / kThreads; ++i) {
+                    const int e = kThreads * i + threadIdx.x;
                     if (e < 16 * MT * kLanes)
-                        bring(buffer(xs, rows * blocks), e / kLanes * blocks + e % kLanes * 16, slot + kRows * kBytes + i * 4096 + wave * 1024, at);
+                        bring(buffer(xs, rows * blocks), e / kLanes * blocks + e % kLanes * 16, slot + kRows * kBytes + (kWaves * i + wave) * 1024, at);
                 }
             }
         } else {
@@ -202,7 +221,8 @@ __global__ __launch_bounds__(256) void mx_stream_kernel(const void* __restrict__
     // The chunk's eight blocks in two instructions: lane group g has the blocks 2 g and 2 g + 1, whose scales are next to each other.
     // Where a lane's pieces are for the first, from a fragment's first row on; for the second they are a piece (e2m1, and the
     // weight) or two (e4m3) on, before the swizzle.
-    const int w_row = wave * (kRows / 4) + lo, x_own = RAW ? (lo < rows ? lo : rows - 1) : lo;
+    const int own = wave & 3, mine = wave >> 2;      // quarter of the weight rows; of two fours the instruction along k
+    const int w_row = own * (kRows / 4) + lo, x_own = RAW ? (lo < rows ? lo : rows - 1) : lo;
     const int w_at = w_row * 128 + swizzle(lo, 2 * hi) * 16;
     const int x_piece = kFour ? 2 * hi : 4 * (hi >> 1) + (hi & 1);
     const int x_at = (RAW ? G::kFixed + x_own * r_bytes : G::kXAt + lo * 128) + swizzle(x_own, x_piece) * 16;
@@ -260,8 +280,9 @@ __global__ __launch_bounds__(256) void mx_stream_kernel(const void* __restrict__
                 for (int i = 0; i < kWT; ++i) acc[i][j] = mfma<FORMAT, h>(a[i], x0, x1, acc[i][j], as[i], bs[j]);
             }
         };
-        half(Const<0>());
-        half(Const<1>());
+        if constexpr (G::kFours == 1) half(Const<0>()), half(Const<1>());
+        else if (mine == 0) half(Const<0>());
+        else half(Const<1>());
         if (begins) put_scales(g + 1);
         s_at += 8, ring = ring == 2 ? 0 : ring + 1;
         if (--left == 0) ++g;
@@ -271,12 +292,28 @@ __global__ __launch_bounds__(256) void mx_stream_kernel(const void* __restrict__
 #pragma unroll 1
     for (; c < c1; ++c) chunk(Const<0>(), c);
     __builtin_amdgcn_s_waitcnt(0x0F70);              // vmcnt(0): no request is on its way to LDS that is another workgroup's by then
+    if constexpr (G::kFours == 2) {
+        __syncthreads();
+        f32x4* meet = reinterpret_cast<f32x4*>(s_mem) + own * (kWT * MT * 64) + lane;
+        if (mine == 1) {
+#pragma unroll
+            for (int j = 0; j < MT; ++j)
+#pragma unroll
+                for (int i = 0; i < kWT; ++i) meet[(j * kWT + i) * 64] = acc[i][j];
+        }
+        __syncthreads();
+        if (mine == 1) return;
+#pragma unroll
+        for (int j = 0; j < MT; ++j)
+#pragma unroll
+            for (int i = 0; i < kWT; ++i) acc[i][j] += meet[(j * kWT + i) * 64];
+    }
     const int64_t pitch = (int64_t)gridDim.x * kRows;
 #pragma unroll
     for (int j = 0; j < MT; ++j)
 #pragma unroll
         for (int i = 0; i < kWT; ++i) {
-            const int m = 16 * j + lo, n = n0 + wave * (kRows / 4) + 16 * i + 4 * hi;
+            const int m = 16 * j + lo, n = n0 + own * (kRows / 4) + 16 * i + 4 * hi;
             if (m >= rows || n >= N) continue;
             if (gridDim.y > 1) *reinterpret_cast<f32x4*>(sums + ((int64_t)split * rows + m) * pitch + n) = acc[i][j];
             else store_sums<T>(acc[i][j], y, bias, m, n, N);
@@ -304,20 +341,20 @@ __global__ __launch_bounds__(256) void mx_add_splits_kernel(const float* __restr
     store_sums<T>(v, y, bias, m, n, N);
 }
 
-template <typename T, int FORMAT, int MT, bool RAW>
+template <typename T, int FORMAT, int MT, int TW, bool RAW>
 hipError_t launch(const Product& p, hipStream_t stream) {
-    using G = Stream<FORMAT, MT, RAW>;
+    using G = Stream<FORMAT, MT, TW, RAW>;
     using E = typename T::elem;
-    const int blocks = (int)(p.k / kBlock), tiles = (int)cdiv(p.n, G::kRows), splits = stream_splits(p.rows, p.n, p.k, p.format);
+    const int blocks = (int)(p.k / kBlock), tiles = (int)cdiv(p.n, G::kRows), splits = plan_of(p.rows, p.n, p.k).splits;
     const int chunks = (blocks & 7 ? 1 : 0) + (blocks >> 3);
     const int lds = G::kFixed + (RAW ? resident_bytes(FORMAT, (int)p.rows, most_chunks(chunks, blocks, splits, G::kGroup)) : 0);
     if (lds > 64 * 1024)
-        if (const hipError_t e = allow_lds<&mx_stream_kernel<T, FORMAT, MT, RAW>>(160 * 1024); e != hipSuccess) return e;
+        if (const hipError_t e = allow_lds<&mx_stream_kernel<T, FORMAT, MT, TW, RAW>>(160 * 1024); e != hipSuccess) return e;
     const int words = blocks % 4 == 0 && blocks >= G::kBytes && ((reinterpret_cast<uintptr_t>(p.ws) | reinterpret_cast<uintptr_t>(p.xs)) & 3) == 0;
     const E *bias = static_cast<const E*>(p.bias);
     E* y = static_cast<E*>(p.y);
     const int groups = (blocks & 7 ? 1 : 0) + ((blocks >> 3) + G::kGroup - 1) / G::kGroup;
-    const hipError_t e = start(&mx_stream_kernel<T, FORMAT, MT, RAW>, dim3(tiles, splits), G::kThreads, lds, stream, RAW ? p.raw : p.x,
+    const hipError_t e = start(&mx_stream_kernel<T, FORMAT, MT, TW, RAW>, dim3(tiles, splits), G::kThreads, lds, stream, RAW ? p.raw : p.x,
                                p.raw_stride, p.xs, p.w, p.ws, bias, y, p.sums, (int)p.rows, (int)p.n, blocks, words, groups / splits,
                                groups % splits);
     if (e != hipSuccess || splits == 1) return e;
@@ -333,32 +370,24 @@ int stream_product(const Product& p, hipStream_t stream) {
     by_type(p.dtype, p.format, [&](auto t, auto f) {
         using T = decltype(t);
         constexpr int F = decltype(f)::value;
-        if (p.raw) e = launch<T, F, 1, true>(p, stream);
-        else if (sixteens(p.rows) == 1) e = launch<T, F, 1, false>(p, stream);
-        else if (sixteens(p.rows) == 2) e = launch<T, F, 2, false>(p, stream);
-        else if (sixteens(p.rows) == 4) e = launch<T, F, 4, false>(p, stream);
-        else e = launch<T, F, 8, false>(p, stream);
+        const int mt = sixteens(p.rows);
+        if (p.raw) e = launch<T, F, 1, 128, true>(p, stream);
+        else if (mt == 1) e = launch<T, F, 1, 128, false>(p, stream);
+        else if (mt == 2) e = launch<T, F, 2, 128, false>(p, stream);
+        else if (mt == 8) e = launch<T, F, 8, 128, false>(p, stream);
+        else if (plan_of(p.rows, p.n, p.k).weight_rows == 128) e = launch<T, F, 4, 128, false>(p, stream);
+        else e = launch<T, F, 4, 256, false>(p, stream);
     });
     return hip_status("mx_stream_kernel", e);
 }
 
-// As many splits as fill the chip with workgroups that are resident at once, of a group of chunks each at least.
-int stream_splits(int64_t rows, int64_t n, int64_t k, int) {
-    const int mt = sixteens(rows), per = group_chunks(mt);
-    const int64_t tiles = cdiv(n, weight_rows(mt)), blocks = k / kBlock, groups = (blocks & 7 ? 1 : 0) + ((blocks >> 3) + per - 1) / per;
-    int64_t s = 256 * per_cu(mt) / tiles;
-    if (s > groups) s = groups;
-    if (s > 16) s = 16;
-    return s < 1 ? 1 : (int)s;
-}
-size_t stream_sums_bytes(int64_t rows, int64_t n, int64_t k, int format) {
-    const int64_t s = stream_splits(rows, n, k, format);
-    const int64_t tile = weight_rows(sixteens(rows));
-    return s > 1 ? (size_t)(s * rows * cdiv(n, tile) * tile * 4) : 0;
+size_t stream_sums_bytes(int64_t rows, int64_t n, int64_t k) {
+    const Plan p = plan_of(rows, n, k);
+    return p.splits > 1 ? (size_t)(p.splits * rows * cdiv(n, p.weight_rows) * p.weight_rows * 4) : 0;
 }
 int stream_raw_bytes(int64_t rows, int64_t n, int64_t k, int format) {
     const int blocks = (int)(k / kBlock), chunks = (blocks & 7 ? 1 : 0) + (blocks >> 3);
-    return resident_bytes(format, (int)rows, most_chunks(chunks, blocks, stream_splits(rows, n, k, format), group_chunks(1)));
+    return resident_bytes(format, (int)rows, most_chunks(chunks, blocks, plan_of(rows, n, k).splits, group_chunks(1)));
 }
 
 }  // namespace nqx
