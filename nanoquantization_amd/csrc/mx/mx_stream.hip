@@ -1,6 +1,5 @@
 // The product for up to 128 rows of x, where what counts is to stream the packed weight once: 0.53 bytes a value, and all of x
-// per workgroup.  A workgroup has 128 weight rows, or 256 where there is more of x to share, all rows of x and a run of k; a wave
-// takes a quarter.  Operands come to LDS by load-to-LDS in chunks of 256 values of k, whole 128-byte lines of a weight row,
+// per workgroup.  A workgroup has 128 weight rows, all rows of x and a run of k; a wave takes a quarter of the weight rows.  Operands come to LDS by load-to-LDS in chunks of 256 values of k, whole 128-byte lines of a weight row,
 // two chunks ahead of the one that is multiplied; one barrier a chunk.  (x comes from a cache, but its requests return behind the
 // weight's: asked for one chunk ahead a chunk of 64 rows took 2.5 us.)  Where the weight has too few rows for the chip, k is split over workgroups, whose
 // sums go to memory in fp32 and are added, in the order of the splits, by a second kernel.
@@ -12,6 +11,7 @@
 namespace nqx {
 namespace {
 
+constexpr int kRows = 128;      // weight rows of a workgroup
 // By sixteens of rows of x: chunks whose scales come at a time, workgroups that fit a CU's LDS, and how many fours of waves a
 // workgroup has: of two, one has a chunk's first instruction along k and one the second, so that a SIMD has something else to do
 // while a wave waits for LDS.
@@ -25,6 +25,19 @@ int most_chunks(int chunks, int blocks, int splits, int group) {
     return most < chunks ? most : chunks;
 }
 int sixteens(int64_t rows) { return rows <= 16 ? 1 : rows <= 32 ? 2 : rows <= 64 ? 4 : 8; }
+// Splits of k: none where 160 workgroups do without (the sums of splits cost another launch), else as many as fill the chip with
+// workgroups that are resident at once, of a group of chunks and four chunks each at least.  (Workgroups of 256 weight rows would
+// share x among more of them: 41 rows by 25600 x 5120 26.5 us and 24.5 with 128, 64 rows by 4096 x 12288 17.6 and 14.3; eight
+// splits of two chunks instead of four of four, 64 rows by 4096 x 4096, 12.2 and 10.7.)
+int splits_of(int64_t rows, int64_t n, int64_t k) {
+    const int mt = sixteens(rows), per = group_chunks(mt);
+    const int64_t blocks = k / kBlock, groups = (blocks & 7 ? 1 : 0) + ((blocks >> 3) + per - 1) / per, tiles = cdiv(n, kRows);
+    int64_t s = tiles >= 160 ? 1 : 256 * per_cu(mt) / tiles;
+    if (s > groups) s = groups;
+    if (s > (blocks >> 5)) s = blocks >> 5;
+    if (s > 16) s = 16;
+    return s < 1 ? 1 : (int)s;
+}
 // Weight rows of a workgroup, and splits of k: as many as fill the chip with workgroups that are resident at once, of a group of
 // chunks each at least.  With 33 to 64 rows of x 256 weight rows share them, unless 128 do without a split, whose sums would cost
 // another launch.
@@ -41,9 +54,9 @@ Plan plan_of(int64_t rows, int64_t n, int64_t k) {
     return {wide, s < 1 ? 1 : (int)s};
 }
 
-template <int FORMAT, int MT, int TW, bool RAW>
+template <int FORMAT, int MT, bool RAW>
 struct Stream {
-    static constexpr int kRows = TW, kFours = fours(MT), kWaves = 4 * kFours, kThreads = 64 * kWaves, kWT = kRows / 64, kBufs = 3, kGroup = group_chunks(MT), kBytes = 8 * kGroup;     // kBytes: a row's scales of a group
+    static constexpr int kFours = fours(MT), kWaves = 4 * kFours, kThreads = 64 * kWaves, kWT = kRows / 64, kBufs = 3, kGroup = group_chunks(MT), kBytes = 8 * kGroup;     // kBytes: a row's scales of a group
     static constexpr int kHalves = FORMAT == NQX_FP4 ? 1 : 2;          // 128-byte parts of a row of x in a chunk
     static constexpr int kW = kRows * 128, kXHalf = 16 * MT * 128, kX = RAW ? 0 : kHalves * kXHalf, kXAt = kBufs * kW;      // [weight | x]
     static constexpr int kWLoads = kRows / 8 / kWaves, kXAll = RAW ? 0 : 2 * MT * kHalves, kXLoads = (kXAll + kWaves - 1) / kWaves;    // of a wave, 1 KiB each
@@ -60,15 +73,15 @@ __host__ __device__ constexpr int resident_bytes(int format, int rows, int chunk
     return rows * chunks * ((format == NQX_FP4 ? 128 : 256) + 8);
 }
 
-template <typename T, int FORMAT, int MT, int TW, bool RAW>
+template <typename T, int FORMAT, int MT, bool RAW>
 __global__ __launch_bounds__(256 * fours(MT)) void mx_stream_kernel(const void* __restrict__ x, int64_t x_stride, const uint8_t* __restrict__ xs,
                                                         const uint8_t* __restrict__ w, const uint8_t* __restrict__ ws,
                                                         const typename T::elem* __restrict__ bias, typename T::elem* __restrict__ y,
                                                         float* __restrict__ sums, int rows, int N, int blocks, int words, int groups_each,
                                                         int groups_more) {
-    using G = Stream<FORMAT, MT, TW, RAW>;
+    using G = Stream<FORMAT, MT, RAW>;
     constexpr bool kFour = FORMAT == NQX_FP4;
-    constexpr int kRows = G::kRows, kWaves = G::kWaves, kThreads = G::kThreads, kWT = G::kWT, kGroup = G::kGroup, kBytes = G::kBytes;
+    constexpr int kWaves = G::kWaves, kThreads = G::kThreads, kWT = G::kWT, kGroup = G::kGroup, kBytes = G::kBytes;
     extern __shared__ __attribute__((aligned(16))) unsigned char s_mem[];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lo = lane & 15, hi = lane >> 4;
     const int split = blockIdx.y, n0 = blockIdx.x * kRows;
@@ -341,24 +354,24 @@ __global__ __launch_bounds__(256) void mx_add_splits_kernel(const float* __restr
     store_sums<T>(v, y, bias, m, n, N);
 }
 
-template <typename T, int FORMAT, int MT, int TW, bool RAW>
+template <typename T, int FORMAT, int MT, bool RAW>
 hipError_t launch(const Product& p, hipStream_t stream) {
-    using G = Stream<FORMAT, MT, TW, RAW>;
+    using G = Stream<FORMAT, MT, RAW>;
     using E = typename T::elem;
-    const int blocks = (int)(p.k / kBlock), tiles = (int)cdiv(p.n, G::kRows), splits = plan_of(p.rows, p.n, p.k).splits;
+    const int blocks = (int)(p.k / kBlock), tiles = (int)cdiv(p.n, kRows), splits = splits_of(p.rows, p.n, p.k);
     const int chunks = (blocks & 7 ? 1 : 0) + (blocks >> 3);
     const int lds = G::kFixed + (RAW ? resident_bytes(FORMAT, (int)p.rows, most_chunks(chunks, blocks, splits, G::kGroup)) : 0);
     if (lds > 64 * 1024)
-        if (const hipError_t e = allow_lds<&mx_stream_kernel<T, FORMAT, MT, TW, RAW>>(160 * 1024); e != hipSuccess) return e;
+        if (const hipError_t e = allow_lds<&mx_stream_kernel<T, FORMAT, MT, RAW>>(160 * 1024); e != hipSuccess) return e;
     const int words = blocks % 4 == 0 && blocks >= G::kBytes && ((reinterpret_cast<uintptr_t>(p.ws) | reinterpret_cast<uintptr_t>(p.xs)) & 3) == 0;
     const E *bias = static_cast<const E*>(p.bias);
     E* y = static_cast<E*>(p.y);
     const int groups = (blocks & 7 ? 1 : 0) + ((blocks >> 3) + G::kGroup - 1) / G::kGroup;
-    const hipError_t e = start(&mx_stream_kernel<T, FORMAT, MT, TW, RAW>, dim3(tiles, splits), G::kThreads, lds, stream, RAW ? p.raw : p.x,
+    const hipError_t e = start(&mx_stream_kernel<T, FORMAT, MT, RAW>, dim3(tiles, splits), G::kThreads, lds, stream, RAW ? p.raw : p.x,
                                p.raw_stride, p.xs, p.w, p.ws, bias, y, p.sums, (int)p.rows, (int)p.n, blocks, words, groups / splits,
                                groups % splits);
     if (e != hipSuccess || splits == 1) return e;
-    const int pitch = tiles * G::kRows;
+    const int pitch = tiles * kRows;
     return start(&mx_add_splits_kernel<T>, dim3((unsigned)cdiv(p.rows * pitch, 1024)), 256, 0, stream, p.sums, bias, y, (int)p.rows, (int)p.n,
                  pitch, splits);
 }
@@ -371,23 +384,22 @@ int stream_product(const Product& p, hipStream_t stream) {
         using T = decltype(t);
         constexpr int F = decltype(f)::value;
         const int mt = sixteens(p.rows);
-        if (p.raw) e = launch<T, F, 1, 128, true>(p, stream);
-        else if (mt == 1) e = launch<T, F, 1, 128, false>(p, stream);
-        else if (mt == 2) e = launch<T, F, 2, 128, false>(p, stream);
-        else if (mt == 8) e = launch<T, F, 8, 128, false>(p, stream);
-        else if (plan_of(p.rows, p.n, p.k).weight_rows == 128) e = launch<T, F, 4, 128, false>(p, stream);
-        else e = launch<T, F, 4, 256, false>(p, stream);
+        if (p.raw) e = launch<T, F, 1, true>(p, stream);
+        else if (mt == 1) e = launch<T, F, 1, false>(p, stream);
+        else if (mt == 2) e = launch<T, F, 2, false>(p, stream);
+        else if (mt == 4) e = launch<T, F, 4, false>(p, stream);
+        else e = launch<T, F, 8, false>(p, stream);
     });
     return hip_status("mx_stream_kernel", e);
 }
 
 size_t stream_sums_bytes(int64_t rows, int64_t n, int64_t k) {
-    const Plan p = plan_of(rows, n, k);
-    return p.splits > 1 ? (size_t)(p.splits * rows * cdiv(n, p.weight_rows) * p.weight_rows * 4) : 0;
+    const int64_t splits = splits_of(rows, n, k);
+    return splits > 1 ? (size_t)(splits * rows * cdiv(n, kRows) * kRows * 4) : 0;
 }
 int stream_raw_bytes(int64_t rows, int64_t n, int64_t k, int format) {
     const int blocks = (int)(k / kBlock), chunks = (blocks & 7 ? 1 : 0) + (blocks >> 3);
-    return resident_bytes(format, (int)rows, most_chunks(chunks, blocks, plan_of(rows, n, k).splits, group_chunks(1)));
+    return resident_bytes(format, (int)rows, most_chunks(chunks, blocks, splits_of(rows, n, k), group_chunks(1)));
 }
 
 }  // namespace nqx
