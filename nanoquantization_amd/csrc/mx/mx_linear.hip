@@ -28,7 +28,7 @@ Form form_of(int64_t rows, int64_t n, int64_t k) {
     // 12288 7.7 us and 7.1 + 1.7, by 5120 x 25600 18.7 and 12.9 + 1.3; 16 rows, which every 16 weight rows read again, by 2560 x 9728
     // 14.7 and 8 + 2.
     if (rows <= 4 ? n * k <= ((int64_t)64 << 20) : rows <= 16 && rows * n * k <= ((int64_t)128 << 20)) return kSkinny;
-    if (rows <= 128) return kStream;
+    if (rows <= 128 || cdiv(rows, 128) * cdiv(n, 128) <= 256) return kStream;
     return cdiv(rows, 256) * cdiv(n, 256) >= 192 ? kTiles256 : kTiles128;
 }
 // Whether a linear quantises x in the product's own kernel: 16 rows, and room in LDS for what a workgroup keeps of them.

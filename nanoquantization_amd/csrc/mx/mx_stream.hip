@@ -1,4 +1,4 @@
-// The product for up to 128 rows of x, where what counts is to stream the packed weight once: 0.53 bytes a value, and all of x
+// The product for a few rows of x, or few tiles of 128, where what counts is to stream the packed weight once: 0.53 bytes a value, and all of x
 // per workgroup.  A workgroup has 128 weight rows, all rows of x and a run of k; a wave takes a quarter of the weight rows.  Operands come to LDS by load-to-LDS in chunks of 256 values of k, whole 128-byte lines of a weight row,
 // two chunks ahead of the one that is multiplied; one barrier a chunk.  (x comes from a cache, but its requests return behind the
 // weight's: asked for one chunk ahead a chunk of 64 rows took 2.5 us.)  Where the weight has too few rows for the chip, k is split over workgroups, whose
@@ -31,7 +31,7 @@ int sixteens(int64_t rows) { return rows <= 16 ? 1 : rows <= 32 ? 2 : rows <= 64
 // splits of two chunks instead of four of four, 64 rows by 4096 x 4096, 12.2 and 10.7.)
 int splits_of(int64_t rows, int64_t n, int64_t k) {
     const int mt = sixteens(rows), per = group_chunks(mt);
-    const int64_t blocks = k / kBlock, groups = (blocks & 7 ? 1 : 0) + ((blocks >> 3) + per - 1) / per, tiles = cdiv(n, kRows);
+    const int64_t blocks = k / kBlock, groups = (blocks & 7 ? 1 : 0) + ((blocks >> 3) + per - 1) / per, tiles = cdiv(n, kRows) * cdiv(rows, 16 * mt);
     int64_t s = tiles >= 160 ? 1 : 256 * per_cu(mt) / tiles;
     if (s > groups) s = groups;
     if (s > (blocks >> 5)) s = blocks >> 5;
@@ -56,7 +56,9 @@ Plan plan_of(int64_t rows, int64_t n, int64_t k) {
 
 template <int FORMAT, int MT, bool RAW>
 struct Stream {
-    static constexpr int kFours = fours(MT), kWaves = 4 * kFours, kThreads = 64 * kWaves, kWT = kRows / 64, kBufs = 3, kGroup = group_chunks(MT), kBytes = 8 * kGroup;     // kBytes: a row's scales of a group
+    static constexpr int kFours = fours(MT), kWaves = 4 * kFours, kThreads = 64 * kWaves, kBufs = 3, kGroup = group_chunks(MT), kBytes = 8 * kGroup;     // kBytes: a row's scales of a group
+    // fragments of a wave: four waves along the weight rows, or two along them and two along 128 rows of x
+    static constexpr int kAlong = MT == 8 ? 2 : 1, kWT = kRows / 64 * kAlong, kXT = MT / kAlong;
     static constexpr int kHalves = FORMAT == NQX_FP4 ? 1 : 2;          // 128-byte parts of a row of x in a chunk
     static constexpr int kW = kRows * 128, kXHalf = 16 * MT * 128, kX = RAW ? 0 : kHalves * kXHalf, kXAt = kBufs * kW;      // [weight | x]
     static constexpr int kWLoads = kRows / 8 / kWaves, kXAll = RAW ? 0 : 2 * MT * kHalves, kXLoads = (kXAll + kWaves - 1) / kWaves;    // of a wave, 1 KiB each
@@ -64,7 +66,7 @@ struct Stream {
     static constexpr int kNone = kXAt + kBufs * kX;                         // where a wave without a piece of x lets its request go
     static constexpr int kScales = kNone + (kXAll % kWaves ? 1024 : 0), kSlot = (kRows + (RAW ? 0 : 16 * MT)) * kBytes;
     static constexpr int kFixed = kScales + 2 * kSlot;
-    static constexpr int kMeet = kFours == 2 ? 4 * kWT * MT * 1024 : 0;      // bytes of LDS where the two fours' sums meet, in the buffers' place
+    static constexpr int kMeet = kFours == 2 ? 4 * kWT * kXT * 1024 : 0;      // bytes of LDS where the two fours' sums meet, in the buffers' place
     static_assert(kMeet <= kNone, "");
     static_assert(kFixed * per_cu(MT) <= 160 * 1024 , "");
 };
@@ -81,11 +83,12 @@ __global__ __launch_bounds__(256 * fours(MT)) void mx_stream_kernel(const void* 
                                                         int groups_more) {
     using G = Stream<FORMAT, MT, RAW>;
     constexpr bool kFour = FORMAT == NQX_FP4;
-    constexpr int kWaves = G::kWaves, kThreads = G::kThreads, kWT = G::kWT, kGroup = G::kGroup, kBytes = G::kBytes;
+    constexpr int kWaves = G::kWaves, kThreads = G::kThreads, kWT = G::kWT, kXT = G::kXT, kGroup = G::kGroup, kBytes = G::kBytes;
     extern __shared__ __attribute__((aligned(16))) unsigned char s_mem[];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lo = lane & 15, hi = lane >> 4;
     const int split = blockIdx.y, n0 = blockIdx.x * kRows;
-    const int n_rows = N - n0 < kRows ? N - n0 : kRows;
+    const int n_rows = N - n0 < kRows ? N - n0 : kRows, m0 = blockIdx.z * (16 * MT), all_rows = rows;
+    rows = rows - m0 < 16 * MT ? rows - m0 : 16 * MT;
     const uint32_t w_pitch = (uint32_t)blocks * 16, x_pitch = (uint32_t)blocks * (kFour ? 16 : 32);
     // Chunks: the blocks that do not fill one come first (pieces that do not exist are asked for past the buffer's end, which
     // leaves zeros), then the whole ones.  Scales come for a group of chunks at a time, kBytes of a row: for the chunk that is
@@ -95,7 +98,8 @@ __global__ __launch_bounds__(256 * fours(MT)) void mx_stream_kernel(const void* 
     const auto chunk_of = [&](int g) { return g < first ? 0 : min(first + kGroup * (g - first), first + whole); };
     const int c0 = chunk_of(g0), c1 = chunk_of(g1);
 
-    const uint8_t *wb = w + (int64_t)n0 * w_pitch, *wsb = ws + (int64_t)n0 * blocks, *xb = static_cast<const uint8_t*>(x);
+    const uint8_t *wb = w + (int64_t)n0 * w_pitch, *wsb = ws + (int64_t)n0 * blocks, *xb = static_cast<const uint8_t*>(x) + (RAW ? 0 : (int64_t)m0 * x_pitch);
+    if constexpr (!RAW) xs += (int64_t)m0 * blocks;
     const auto buffer = [](const uint8_t* p, uint32_t bytes) {
         return __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(p), 0, bytes, 0x00020000);
     };
@@ -196,11 +200,11 @@ __global__ __launch_bounds__(256 * fours(MT)) void mx_stream_kernel(const void* 
         }
     };
 
-    f32x4 acc[kWT][MT];
+    f32x4 acc[kWT][kXT];
 #pragma unroll
     for (int i = 0; i < kWT; ++i)
 #pragma unroll
-        for (int j = 0; j < MT; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+        for (int j = 0; j < kXT; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
 
     ask_scales(g0);
     load(Const<1>(), c0, 0);
@@ -235,10 +239,11 @@ __global__ __launch_bounds__(256 * fours(MT)) void mx_stream_kernel(const void* 
     // Where a lane's pieces are for the first, from a fragment's first row on; for the second they are a piece (e2m1, and the
     // weight) or two (e4m3) on, before the swizzle.
     const int own = wave & 3, mine = wave >> 2;      // quarter of the weight rows; of two fours the instruction along k
-    const int w_row = own * (kRows / 4) + lo, x_own = RAW ? (lo < rows ? lo : rows - 1) : lo;
+    const int wm = own % (4 / G::kAlong), wn = own / (4 / G::kAlong);
+    const int w_row = wm * (16 * kWT) + lo, x_row = wn * (16 * kXT) + lo, x_own = lo < rows ? lo : rows - 1;
     const int w_at = w_row * 128 + swizzle(lo, 2 * hi) * 16;
     const int x_piece = kFour ? 2 * hi : 4 * (hi >> 1) + (hi & 1);
-    const int x_at = (RAW ? G::kFixed + x_own * r_bytes : G::kXAt + lo * 128) + swizzle(x_own, x_piece) * 16;
+    const int x_at = RAW ? G::kFixed + x_own * r_bytes + swizzle(x_own, x_piece) * 16 : G::kXAt + x_row * 128 + swizzle(lo, x_piece) * 16;
     const auto read = [&](int at) { return *reinterpret_cast<const u32x4*>(s_mem + at); };
     int ring = 0, g = g0, s_at = 0, left = 0;
     const auto chunk = [&](auto partial_, int c) {
@@ -266,13 +271,13 @@ __global__ __launch_bounds__(256 * fours(MT)) void mx_stream_kernel(const void* 
                 return *reinterpret_cast<const uint16_t*>(s_mem + at + 2 * hi);
             }
         };
-        uint32_t as[kWT], bs[MT];
+        uint32_t as[kWT], bs[kXT];
 #pragma unroll
         for (int i = 0; i < kWT; ++i) as[i] = scales(s_at + (w_row + 16 * i) * kBytes);
 #pragma unroll
-        for (int j = 0; j < MT; ++j) {
+        for (int j = 0; j < kXT; ++j) {
             if constexpr (RAW) bs[j] = *reinterpret_cast<const uint16_t*>(s_xs + x_own * chunks * 8 + (c - c0) * 8 + 2 * hi);
-            else bs[j] = scales(s_at + (kRows + 16 * j + lo) * kBytes);
+            else bs[j] = scales(s_at + (kRows + x_row + 16 * j) * kBytes);
         }
         const int wp = ring * G::kW + w_at, xp = x_at + (RAW ? (c - c0) * (kFour ? 128 : 256) : ring * G::kX);
         const auto half = [&](auto h_) {
@@ -281,7 +286,7 @@ __global__ __launch_bounds__(256 * fours(MT)) void mx_stream_kernel(const void* 
 #pragma unroll
             for (int i = 0; i < kWT; ++i) a[i] = read((wp ^ (16 * h)) + i * 2048);
 #pragma unroll
-            for (int j = 0; j < MT; ++j) {
+            for (int j = 0; j < kXT; ++j) {
                 u32x4 x0, x1;
                 if constexpr (kFour) {
                     x0 = x1 = read((xp ^ (16 * h)) + j * 2048);
@@ -307,29 +312,29 @@ __global__ __launch_bounds__(256 * fours(MT)) void mx_stream_kernel(const void* 
     __builtin_amdgcn_s_waitcnt(0x0F70);              // vmcnt(0): no request is on its way to LDS that is another workgroup's by then
     if constexpr (G::kFours == 2) {
         __syncthreads();
-        f32x4* meet = reinterpret_cast<f32x4*>(s_mem) + own * (kWT * MT * 64) + lane;
+        f32x4* meet = reinterpret_cast<f32x4*>(s_mem) + own * (kWT * kXT * 64) + lane;
         if (mine == 1) {
 #pragma unroll
-            for (int j = 0; j < MT; ++j)
+            for (int j = 0; j < kXT; ++j)
 #pragma unroll
                 for (int i = 0; i < kWT; ++i) meet[(j * kWT + i) * 64] = acc[i][j];
         }
         __syncthreads();
         if (mine == 1) return;
 #pragma unroll
-        for (int j = 0; j < MT; ++j)
+        for (int j = 0; j < kXT; ++j)
 #pragma unroll
             for (int i = 0; i < kWT; ++i) acc[i][j] += meet[(j * kWT + i) * 64];
     }
     const int64_t pitch = (int64_t)gridDim.x * kRows;
 #pragma unroll
-    for (int j = 0; j < MT; ++j)
+    for (int j = 0; j < kXT; ++j)
 #pragma unroll
         for (int i = 0; i < kWT; ++i) {
-            const int m = 16 * j + lo, n = n0 + own * (kRows / 4) + 16 * i + 4 * hi;
+            const int m = x_row + 16 * j, n = n0 + wm * (16 * kWT) + 16 * i + 4 * hi;
             if (m >= rows || n >= N) continue;
-            if (gridDim.y > 1) *reinterpret_cast<f32x4*>(sums + ((int64_t)split * rows + m) * pitch + n) = acc[i][j];
-            else store_sums<T>(acc[i][j], y, bias, m, n, N);
+            if (gridDim.y > 1) *reinterpret_cast<f32x4*>(sums + ((int64_t)split * all_rows + m0 + m) * pitch + n) = acc[i][j];
+            else store_sums<T>(acc[i][j], y, bias, m0 + m, n, N);
         }
 }
 
@@ -367,7 +372,7 @@ hipError_t launch(const Product& p, hipStream_t stream) {
     const E *bias = static_cast<const E*>(p.bias);
     E* y = static_cast<E*>(p.y);
     const int groups = (blocks & 7 ? 1 : 0) + ((blocks >> 3) + G::kGroup - 1) / G::kGroup;
-    const hipError_t e = start(&mx_stream_kernel<T, FORMAT, MT, RAW>, dim3(tiles, splits), G::kThreads, lds, stream, RAW ? p.raw : p.x,
+    const hipError_t e = start(&mx_stream_kernel<T, FORMAT, MT, RAW>, dim3(tiles, splits, (unsigned)cdiv(p.rows, 16 * MT)), G::kThreads, lds, stream, RAW ? p.raw : p.x,
                                p.raw_stride, p.xs, p.w, p.ws, bias, y, p.sums, (int)p.rows, (int)p.n, blocks, words, groups / splits,
                                groups % splits);
     if (e != hipSuccess || splits == 1) return e;
