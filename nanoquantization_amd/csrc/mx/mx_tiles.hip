@@ -4,8 +4,9 @@
 // an e4m3 one.  (What feeds a tile is the L2, and it takes requests, not bytes: with 64 bytes of a row at a time 8192 x 8192 x 8192
 // in 4 bits was 334 us, 246 without a matrix instruction.)  Two chunks are in LDS.  A wave reads the fragments of a step while the
 // matrix cores have the one before, so at a chunk's last step nobody needs its buffer any more: there is the one barrier of a
-// chunk, which also says that the next one has landed, and behind it the requests for the chunk after that go out, some a step;
-// they have as long as a chunk's products take.
+// chunk, which also says that the next one has landed, and behind it the requests for the chunk after that go out, over half a
+// chunk's products (over three quarters of them 8192 cubed takes 289 us instead of 277, in 8 bits 433 and 425: the last ones are
+// waited for).
 #include "../pingpong.hpp"
 #include "mx_linear.hpp"
 
@@ -234,13 +235,13 @@ __global__ __launch_bounds__(256, (S == 256 ? 1 : 2)) void mx_tiles_kernel(
                 read_scales(c + 1, an, bn);
             }
             const int at = ks == 3 ? ((c + 1) & 1) * G::kPart : (c & 1) * G::kPart, k16 = ks == 3 ? 0 : (ks + 1) * 16;
-            constexpr int kSlots = 3 * XT;           // requests for chunk c + 2 (or those still to make for c + 1): steps 3, 0 and 1
+            constexpr int kSlots = 2 * XT;           // requests for chunk c + 2 (or those still to make for c + 1): steps 3 and 0
 #pragma unroll
             for (int j = 0; j < XT; ++j) {
                 // the next step's fragments
                 b[1 - p][j] = read(((at + x_at) ^ k16) + j * R * 128);
                 a[1 - p][j] = read(((at + w_at) ^ k16) + j * R * 128);
-                if constexpr (ks != 2) {
+                if constexpr (ks == 3 || ks == 0) {
                     constexpr int s0 = ks == 3 ? 0 : XT * (ks + 1);
                     const int target = ks == 3 ? c + 2 : c + 1;
 #pragma unroll
@@ -295,7 +296,7 @@ __global__ __launch_bounds__(256, (S == 256 ? 1 : 2)) void mx_tiles_kernel(
             for (int i = 0; i < WT; ++i) read_w(i, 0, s);
             read_x(b[0], 0, 0, s), read_x(b[1], 1, 0, s);
         }
-        constexpr int kAll = G::kLoads + G::kLoads / 2, kSpread = XT / 2, kStep = (kAll + kSpread - 1) / kSpread;
+        constexpr int kAll = G::kLoads + G::kLoads / 2, kSpread = XT >= 8 ? 3 : 2, kStep = (kAll + kSpread - 1) / kSpread;
 #pragma unroll 1
         for (int t = 0; t < halves; ++t) {
             if ((t & 1) == 0) scales_ahead(t >> 1);
