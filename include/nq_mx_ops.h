@@ -7,16 +7,18 @@
  *   NQX_FP8  e4m3 (largest 448), one byte each.
  * e is the smallest exponent with which the block's largest magnitude, rounded to the nearest element, is not past the
  * largest element, and at least -127: no value is off by more than half a step.  A block with an infinity or a NaN has the
- * scale byte 255 and codes 0, and stands for NaN.  Magnitudes from 1.75 * 2^127 on may round up to 2^128, past fp32.  (Element and scale types are those of the OCP Microscaling Formats
- * specification; its own scale, without the exponent's step up, saturates the largest values and is off by more: normal
- * values 0.115 instead of 0.112 in e2m1 and 0.0293 instead of 0.0266 in e4m3, relative.)
+ * scale byte 255 and codes 0, and stands for NaN.  Magnitudes from 1.75 * 2^127 on may round up to 2^128, past fp32.
+ * (Element and scale types are those of the OCP Microscaling Formats specification; its own scale, without the exponent's
+ * step up, saturates the largest values and is off by more: normal values 0.115 instead of 0.112 in e2m1 and 0.0293 instead
+ * of 0.0266 in e4m3, relative.)
  *
  * Layout: codes [rows, k / 2] (NQX_FP4) or [rows, k] (NQX_FP8), scales [rows, k / 32], both uint8 and dense row-major;
  * k % 32 == 0.  Weights are NQX_FP4, [n, k / 2] and [n, k / 32]: the rows of a torch Linear weight.
  *
  * Conventions: device pointers on the current HIP device, 16-byte aligned except scales and biases (any address of their
  * type).  `dtype` is the type of the unquantised tensors of a call.  Strides are in elements, rows start on 16-byte
- * boundaries.  `stream` is a hipStream_t as void*; calls are asynchronous on it, allocate nothing and can be captured.
+ * boundaries.  A call has fewer than 2^36 values of x and k <= 2^30, a product rows <= 2^20 and n <= 2^29; 0 rows (and n = 0)
+ * are nothing to do, and no pointer is looked at then.  `stream` is a hipStream_t as void*; calls are asynchronous on it, allocate nothing and can be captured.
  * Inputs are not written.  Results do not depend on what else runs, and equal calls give equal bits.  The return value is 0
  * or an NQX_ERR code, nqx_last_error() holds the message of the calling thread's last failure.  The reference has no
  * counterpart: its linears are 4-bit integers with 16-bit activations. */
@@ -65,7 +67,8 @@ const char* nqx_linear_form(int64_t rows, int64_t n, int64_t k, int dtype, int f
 
 /* total [rows, k] = x + delta, rounded to dtype (delta NULL: total is x, and may be NULL, else it is written too), and
  * codes, scales of total * rsqrt(mean(total^2) + eps) * weight, computed in fp32 from the rounded sum.  x, delta and total
- * are rows x_stride, delta_stride and k apart; total may be x or delta where their rows are k apart.  k <= 16384. */
+ * are rows x_stride, delta_stride and k apart; total may be x or delta where their rows are k apart.  Squares past fp32 give a
+ * mean of infinity, and zeros.  k <= 16384, rows < 2^24. */
 int nqx_add_rmsnorm(const void* x, int64_t x_stride, const void* delta, int64_t delta_stride, const void* weight,
                     void* total, uint8_t* codes, uint8_t* scales, int64_t rows, int64_t k, float eps, int dtype, int format,
                     void* stream);

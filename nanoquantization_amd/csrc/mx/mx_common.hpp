@@ -49,6 +49,12 @@ struct F32 {
     static __device__ __forceinline__ float from_f32(float f) { return f; }
 };
 
+// (By value: a bit_cast of a vector's element takes the vector's first.)
+template <typename V>
+__device__ __forceinline__ V as(uint32_t bits) {
+    return __builtin_bit_cast(V, bits);
+}
+
 // Eight consecutive elements, 16-byte accesses.
 template <typename T>
 __device__ __forceinline__ void load8(const typename T::elem* p, float (&v)[8]) {
@@ -122,15 +128,100 @@ __device__ __forceinline__ u32x2 encode8(const float (&v)[8], uint32_t byte) {
         return u32x2{__builtin_bit_cast(uint32_t, a), __builtin_bit_cast(uint32_t, b)};
     }
 }
-// One lane's part of a quantised row: eight values, number `at` of the tensor's eights.  All four lanes of a block call it.
+// Eight 16-bit values as they are in memory: magnitudes two at a time, and conversions that take the pairs.
+template <typename T>
+__device__ __forceinline__ uint32_t magnitude_bits(u32x4 w) {
+    typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
+    u16x2 m = __builtin_bit_cast(u16x2, w[0] & 0x7FFF7FFFu);
+#pragma unroll
+    for (int i = 1; i < 4; ++i) m = __builtin_elementwise_max(m, __builtin_bit_cast(u16x2, w[i] & 0x7FFF7FFFu));
+    return __builtin_bit_cast(uint32_t, T::to_f32(m[0] > m[1] ? m[0] : m[1]));
+}
+template <typename T, int FORMAT>
+__device__ __forceinline__ u32x2 encode8(u32x4 w, uint32_t byte) {
+    if (byte == 255) return u32x2{0u, 0u};
+    const float scale = power(byte);
+    if constexpr (FORMAT == NQX_FP4) {
+        uint32_t c = 0;
+        if constexpr (T::id == NQX_BF16) {
+            c = __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(c, as<bf16x2>(w[0]), scale, 0);
+            c = __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(c, as<bf16x2>(w[1]), scale, 1);
+            c = __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(c, as<bf16x2>(w[2]), scale, 2);
+            c = __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(c, as<bf16x2>(w[3]), scale, 3);
+        } else {
+            c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f16(c, as<f16x2>(w[0]), scale, 0);
+            c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f16(c, as<f16x2>(w[1]), scale, 1);
+            c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f16(c, as<f16x2>(w[2]), scale, 2);
+            c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f16(c, as<f16x2>(w[3]), scale, 3);
+        }
+        return u32x2{c, 0u};
+    } else {
+        i16x2 a = {0, 0}, b = {0, 0};
+        if constexpr (T::id == NQX_BF16) {
+            a = __builtin_amdgcn_cvt_scalef32_pk_fp8_bf16(a, as<bf16x2>(w[0]), scale, false);
+            a = __builtin_amdgcn_cvt_scalef32_pk_fp8_bf16(a, as<bf16x2>(w[1]), scale, true);
+            b = __builtin_amdgcn_cvt_scalef32_pk_fp8_bf16(b, as<bf16x2>(w[2]), scale, false);
+            b = __builtin_amdgcn_cvt_scalef32_pk_fp8_bf16(b, as<bf16x2>(w[3]), scale, true);
+        } else {
+            a = __builtin_amdgcn_cvt_scalef32_pk_fp8_f16(a, as<f16x2>(w[0]), scale, false);
+            a = __builtin_amdgcn_cvt_scalef32_pk_fp8_f16(a, as<f16x2>(w[1]), scale, true);
+            b = __builtin_amdgcn_cvt_scalef32_pk_fp8_f16(b, as<f16x2>(w[2]), scale, false);
+            b = __builtin_amdgcn_cvt_scalef32_pk_fp8_f16(b, as<f16x2>(w[3]), scale, true);
+        }
+        return u32x2{__builtin_bit_cast(uint32_t, a), __builtin_bit_cast(uint32_t, b)};
+    }
+}
+// One lane's part of a quantised row: its codes and, of the four lanes of a block, the first one's scale, number `at` of the
+// tensor's eights.
+template <int FORMAT>
+__device__ __forceinline__ void put8(u32x2 code, uint32_t byte, uint8_t* codes, uint8_t* scales, int64_t at) {
+    if constexpr (FORMAT == NQX_FP4) reinterpret_cast<uint32_t*>(codes)[at] = code.x;
+    else reinterpret_cast<u32x2*>(codes)[at] = code;
+    if ((at & 3) == 0) scales[at >> 2] = (uint8_t)byte;
+}
+// All four lanes of a block call it.
 template <int FORMAT>
 __device__ __forceinline__ void quantize8(const float (&v)[8], uint8_t* codes, uint8_t* scales, int64_t at) {
     const uint32_t byte = scale_byte<FORMAT>(max_of_block(magnitude_bits(v)));
-    const u32x2 w = encode8<FORMAT>(v, byte);
-    if constexpr (FORMAT == NQX_FP4) reinterpret_cast<uint32_t*>(codes)[at] = w.x;
-    else reinterpret_cast<u32x2*>(codes)[at] = w;
-    if ((at & 3) == 0) scales[at >> 2] = (uint8_t)byte;
+    put8<FORMAT>(encode8<FORMAT>(v, byte), byte, codes, scales, at);
 }
+// Eight values at p, quantised: of 16-bit types without a detour over fp32, the same codes.
+template <typename T, int FORMAT>
+struct Eight {
+    u32x4 w[T::id == NQX_F32 ? 2 : 1];
+    __device__ __forceinline__ void load(const typename T::elem* p) {
+        w[0] = reinterpret_cast<const u32x4*>(p)[0];
+        if constexpr (T::id == NQX_F32) w[1] = reinterpret_cast<const u32x4*>(p)[1];
+    }
+    __device__ __forceinline__ void clear() {
+        w[0] = u32x4{0u, 0u, 0u, 0u};
+        if constexpr (T::id == NQX_F32) w[1] = w[0];
+    }
+    __device__ __forceinline__ void floats(float (&v)[8]) const {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            if constexpr (T::id == NQX_F32) {
+                v[i] = as<float>(w[0][i]), v[4 + i] = as<float>(w[1][i]);
+            } else {
+                const uint32_t u = w[0][i];
+                v[2 * i] = T::to_f32((uint16_t)(u & 0xFFFFu)), v[2 * i + 1] = T::to_f32((uint16_t)(u >> 16));
+            }
+        }
+    }
+    // the codes; `byte`: the scale
+    __device__ __forceinline__ u32x2 encode(uint32_t& byte) const {
+        if constexpr (T::id == NQX_F32) {
+            float v[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) v[i] = as<float>(w[i / 4][i % 4]);
+            byte = scale_byte<FORMAT>(max_of_block(magnitude_bits(v)));
+            return encode8<FORMAT>(v, byte);
+        } else {
+            byte = scale_byte<FORMAT>(max_of_block(magnitude_bits<T>(w[0])));
+            return encode8<T, FORMAT>(w[0], byte);
+        }
+    }
+};
 
 // ---- host ----------------------------------------------------------------------------------------------------------------
 int refuse(int status, const char* fmt, ...);

@@ -8,7 +8,7 @@ namespace {
 int check_product(const char* fn, int64_t rows, int64_t n, int64_t k, int dtype, int format) {
     if (int s = check_types(fn, rows, k, dtype, format)) return s;
     if (n < 0) return refuse(NQX_ERR_ARG, "%s: n must not be negative (%lld)", fn, (long long)n);
-    if (n > ((int64_t)1 << 30) || rows > ((int64_t)1 << 20))
+    if (n > ((int64_t)1 << 29) || rows > ((int64_t)1 << 20))
         return refuse(NQX_ERR_UNSUPPORTED, "%s: problem too large (rows=%lld n=%lld)", fn, (long long)rows, (long long)n);
     return NQX_OK;
 }

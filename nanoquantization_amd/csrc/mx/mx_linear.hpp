@@ -44,19 +44,23 @@ template <typename T>
 __device__ __forceinline__ void store_sums(f32x4 v, typename T::elem* y, const typename T::elem* bias, int64_t row, int64_t n,
                                            int64_t N) {
     typename T::elem* to = y + row * N + n;
-    if (bias) {
+    if (n + 4 <= N) {
+        if (bias) {
 #pragma unroll
-        for (int r = 0; r < 4; ++r)
-            if (n + r < N) v[r] += T::to_f32(bias[n + r]);
+            for (int r = 0; r < 4; ++r) v[r] += T::to_f32(bias[n + r]);
+        }
+        // any address of the type
+        if constexpr (sizeof(typename T::elem) == 4) {
+            __builtin_memcpy(to, &v, 16);
+        } else {
+            const u32x2 w = {T::pack2(v[0], v[1]), T::pack2(v[2], v[3])};
+            __builtin_memcpy(to, &w, 8);
+        }
+        return;
     }
-    if ((N & 3) == 0) {          // then n + 3 < N, and the four are aligned
-        if constexpr (sizeof(typename T::elem) == 4) *reinterpret_cast<f32x4*>(to) = v;
-        else *reinterpret_cast<u32x2*>(to) = u32x2{T::pack2(v[0], v[1]), T::pack2(v[2], v[3])};
-    } else {
 #pragma unroll
-        for (int r = 0; r < 4; ++r)
-            if (n + r < N) to[r] = T::from_f32(v[r]);
-    }
+    for (int r = 0; r < 3; ++r)
+        if (n + r < N) to[r] = T::from_f32(bias ? v[r] + T::to_f32(bias[n + r]) : v[r]);
 }
 
 int skinny_product(const Product& p, hipStream_t stream);       // at most 16 rows of raw x

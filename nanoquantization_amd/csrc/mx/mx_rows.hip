@@ -1,6 +1,8 @@
 // Row kernels of the microscaled formats: quantise, dequantise, residual addition + RMSNorm, SiLU(gate) * up.  All are
-// bound by memory: a lane takes eight consecutive values in one or two 16-byte loads, the four lanes of a block agree on
-// the largest magnitude by two DPP moves, and codes leave in 4- or 8-byte stores, whole lines a wave.
+// bound by memory: a lane takes eight consecutive values in one or two 16-byte loads, several eights at once, the four lanes of
+// a block agree on the largest magnitude by two DPP moves, and codes leave in 4- or 8-byte stores, whole lines a wave.  In bf16,
+// 25600 x 5120: quantise to e2m1 68 us (4.9 TB/s; 88 to e4m3, 4.5), dequantise 53 and 58 (6.3 and 6.8 with the codes still in
+// the last cache); 8192 x 5120: sum, norm and e4m3 63 us (4.7 TB/s).  A large copy reaches 5.2.
 #include "mx_common.hpp"
 
 namespace nqx {
@@ -8,46 +10,75 @@ namespace {
 
 constexpr int kThreads = 256;
 
-// A grid-stride loop over the tensor's eights: fn(row, column in eights, number).
-template <typename F>
-__device__ __forceinline__ void each_eight(int64_t count, uint32_t per_row, F&& fn) {
-    for (int64_t at = (int64_t)blockIdx.x * kThreads + threadIdx.x; at < count; at += (int64_t)gridDim.x * kThreads) {
-        const int64_t row = at / per_row;
-        fn(row, (uint32_t)(at - row * per_row), at);
+// A workgroup takes kMany * 256 consecutive eights of the tensor, a lane kMany of them, all loaded before the first is used.
+constexpr int kMany = 4;
+
+// Where eight `at` of rows `stride` values apart begins.  Dense rows need no division, which would cost a launch of a few rows a
+// microsecond.
+__device__ __forceinline__ int64_t place(int64_t at, int64_t stride, uint32_t per_row) {
+    if (stride == (int64_t)per_row * 8) return at * 8;
+    if ((at >> 32) == 0) {
+        const uint32_t row = (uint32_t)at / per_row;
+        return row * stride + (int64_t)((uint32_t)at - row * per_row) * 8;
     }
+    const int64_t row = at / per_row;
+    return row * stride + (at - row * per_row) * 8;
 }
 
 template <typename T, int FORMAT>
 __global__ __launch_bounds__(kThreads) void mx_quantize_kernel(const typename T::elem* __restrict__ x, int64_t stride,
                                                                uint8_t* __restrict__ codes, uint8_t* __restrict__ scales,
                                                                int64_t count, uint32_t per_row) {
-    each_eight(count, per_row, [&](int64_t row, uint32_t column, int64_t at) {
-        float v[8];
-        load8<T>(x + row * stride + (int64_t)column * 8, v);
-        quantize8<FORMAT>(v, codes, scales, at);
-    });
+    const int64_t first = (int64_t)blockIdx.x * (kMany * kThreads) + threadIdx.x;
+    Eight<T, FORMAT> e[kMany];
+#pragma unroll
+    for (int u = 0; u < kMany; ++u) {
+        const int64_t at = first + u * kThreads;
+        if (at < count) e[u].load(x + place(at, stride, per_row));
+    }
+#pragma unroll
+    for (int u = 0; u < kMany; ++u) {
+        const int64_t at = first + u * kThreads;
+        if (at >= count) break;              // whole blocks: count is a multiple of four
+        uint32_t byte;
+        const u32x2 code = e[u].encode(byte);
+        put8<FORMAT>(code, byte, codes, scales, at);
+    }
 }
 
 template <typename T, int FORMAT>
 __global__ __launch_bounds__(kThreads) void mx_dequantize_kernel(const uint8_t* __restrict__ codes,
                                                                  const uint8_t* __restrict__ scales,
                                                                  typename T::elem* __restrict__ y, int64_t count) {
-    for (int64_t at = (int64_t)blockIdx.x * kThreads + threadIdx.x; at < count; at += (int64_t)gridDim.x * kThreads) {
-        const float scale = power(scales[at >> 2]);
+    const int64_t first = (int64_t)blockIdx.x * (kMany * kThreads) + threadIdx.x;
+    u32x2 w[kMany];
+    uint32_t byte[kMany];
+#pragma unroll
+    for (int u = 0; u < kMany; ++u) {
+        const int64_t at = first + u * kThreads;
+        w[u] = u32x2{0u, 0u}, byte[u] = 0;
+        if (at >= count) continue;
+        if constexpr (FORMAT == NQX_FP4) w[u].x = reinterpret_cast<const uint32_t*>(codes)[at];
+        else w[u] = reinterpret_cast<const u32x2*>(codes)[at];
+        byte[u] = scales[at >> 2];
+    }
+#pragma unroll
+    for (int u = 0; u < kMany; ++u) {
+        const int64_t at = first + u * kThreads;
+        if (at >= count) break;
+        const float scale = power(byte[u]);
         float v[8];
         // element times power of two is exact in fp32
         if constexpr (FORMAT == NQX_FP4) {
-            const uint32_t w = reinterpret_cast<const uint32_t*>(codes)[at];
             const auto two = [&](auto sel) {
-                const auto p = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, 1.0f, decltype(sel)::value);
+                const auto p = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w[u].x, 1.0f, decltype(sel)::value);
                 v[2 * decltype(sel)::value] = p[0] * scale, v[2 * decltype(sel)::value + 1] = p[1] * scale;
             };
             two(Const<0>()), two(Const<1>()), two(Const<2>()), two(Const<3>());
         } else {
-            const u32x2 w = reinterpret_cast<const u32x2*>(codes)[at];
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
-                const auto a = __builtin_amdgcn_cvt_pk_f32_fp8(w[i], false), b = __builtin_amdgcn_cvt_pk_f32_fp8(w[i], true);
+                const auto a = __builtin_amdgcn_cvt_pk_f32_fp8(w[u][i], false), b = __builtin_amdgcn_cvt_pk_f32_fp8(w[u][i], true);
                 v[4 * i] = a[0] * scale, v[4 * i + 1] = a[1] * scale, v[4 * i + 2] = b[0] * scale, v[4 * i + 3] = b[1] * scale;
             }
         }
@@ -64,26 +95,28 @@ __global__ __launch_bounds__(kThreads) void mx_add_rmsnorm_kernel(const typename
                                                                   uint8_t* __restrict__ scales, uint32_t per_row, float eps) {
     __shared__ float s_sum[kThreads / 64];
     const int64_t row = blockIdx.x;
+    Eight<T, FORMAT> in[CHUNKS], add[CHUNKS];
+#pragma unroll
+    for (int c = 0; c < CHUNKS; ++c) {
+        const uint32_t column = c * kThreads + threadIdx.x;
+        in[c].clear(), add[c].clear();
+        if (column < per_row) {
+            in[c].load(x + row * x_stride + (int64_t)column * 8);
+            if (delta) add[c].load(delta + row * delta_stride + (int64_t)column * 8);
+        }
+    }
     float v[CHUNKS][8], ss = 0.f;
 #pragma unroll
     for (int c = 0; c < CHUNKS; ++c) {
         const uint32_t column = c * kThreads + threadIdx.x;
+        in[c].floats(v[c]);
+        if (delta) {
+            float d[8];
+            add[c].floats(d);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) v[c][e] = 0.f;
-        if (column < per_row) load8<T>(x + row * x_stride + (int64_t)column * 8, v[c]);
-    }
-#pragma unroll
-    for (int c = 0; c < CHUNKS; ++c) {
-        const uint32_t column = c * kThreads + threadIdx.x;
-        if (column < per_row) {
-            if (delta) {
-                float d[8];
-                load8<T>(delta + row * delta_stride + (int64_t)column * 8, d);
-#pragma unroll
-                for (int e = 0; e < 8; ++e) v[c][e] = T::to_f32(T::from_f32(v[c][e] + d[e]));
-            }
-            if (total) store8<T>(total + (row * per_row + column) * 8, v[c]);
+            for (int e = 0; e < 8; ++e) v[c][e] = T::to_f32(T::from_f32(v[c][e] + d[e]));
         }
+        if (total && column < per_row) store8<T>(total + (row * per_row + column) * 8, v[c]);
 #pragma unroll
         for (int e = 0; e < 8; ++e) ss = __builtin_fmaf(v[c][e], v[c][e], ss);
     }
@@ -108,26 +141,44 @@ __global__ __launch_bounds__(kThreads) void mx_add_rmsnorm_kernel(const typename
     }
 }
 
+// gate / (1 + exp(-gate)) * up.  exp(-g) is 2^t 2^r, t = -g log2(e) rounded and r what that and the constant lost: without r the
+// relative error grows with |g|.  (2^r as a factor of its own near 1: where 2^t is infinite a sum could be inf - inf.)  The
+// reciprocal is off by a step of fp32 at most, a division would be by half of one and takes ten times as long (8192 x 12288 bf16
+// to e2m1 is 104 us, 4.4 TB/s, and was 116 with expf and a division).  Past 100 the exponential is infinite or does not change 1.
+__device__ __forceinline__ float silu_mul(float gate, float up) {
+    constexpr float kHigh = 1.44269502f, kLow = 1.92596303e-8f, kLn2 = 0.693147182f;
+    const float g = -fminf(fmaxf(gate, -100.f), 100.f), t = g * kHigh;
+    const float r = __builtin_fmaf(g, kLow, __builtin_fmaf(g, kHigh, -t));
+    const float e = __builtin_amdgcn_exp2f(t) * __builtin_fmaf(r, kLn2, 1.0f);
+    return gate * __builtin_amdgcn_rcpf(1.0f + e) * up;
+}
+
 template <typename T, int FORMAT>
 __global__ __launch_bounds__(kThreads) void mx_silu_mul_kernel(const typename T::elem* __restrict__ gate, int64_t gate_stride,
                                                                const typename T::elem* __restrict__ up, int64_t up_stride,
                                                                uint8_t* __restrict__ codes, uint8_t* __restrict__ scales,
                                                                int64_t count, uint32_t per_row) {
-    each_eight(count, per_row, [&](int64_t row, uint32_t column, int64_t at) {
-        float g[8], u[8];
-        load8<T>(gate + row * gate_stride + (int64_t)column * 8, g);
-        load8<T>(up + row * up_stride + (int64_t)column * 8, u);
+    constexpr int kTwo = 2;                  // eights of a lane: they are two loads each
+    const int64_t first = (int64_t)blockIdx.x * (kTwo * kThreads) + threadIdx.x;
+    Eight<T, FORMAT> g[kTwo], u[kTwo];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) g[e] = g[e] / (1.0f + expf(-g[e])) * u[e];
-        quantize8<FORMAT>(g, codes, scales, at);
-    });
+    for (int i = 0; i < kTwo; ++i) {
+        const int64_t at = first + i * kThreads;
+        if (at < count) g[i].load(gate + place(at, gate_stride, per_row)), u[i].load(up + place(at, up_stride, per_row));
+    }
+#pragma unroll
+    for (int i = 0; i < kTwo; ++i) {
+        const int64_t at = first + i * kThreads;
+        if (at >= count) break;
+        float a[8], b[8];
+        g[i].floats(a), u[i].floats(b);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) a[e] = silu_mul(a[e], b[e]);
+        quantize8<FORMAT>(a, codes, scales, at);
+    }
 }
 
-// Enough workgroups to fill the chip several times over, each with a few rounds of the loop at the largest sizes.
-int grid_for(int64_t eights) {
-    const int64_t g = cdiv(eights, kThreads);
-    return (int)(g < 65536 ? g : 65536);
-}
+unsigned groups(int64_t eights, int of_a_lane) { return (unsigned)cdiv(eights, of_a_lane * kThreads); }
 
 }  // namespace
 
@@ -137,7 +188,7 @@ int quantize(const void* x, int64_t x_stride, uint8_t* codes, uint8_t* scales, i
     by_type(dtype, format, [&](auto t, auto f) {
         using T = decltype(t);
         const int64_t count = rows * (k / kLane);
-        e = start(&mx_quantize_kernel<T, decltype(f)::value>, dim3(grid_for(count)), kThreads, 0, stream, 
+        e = start(&mx_quantize_kernel<T, decltype(f)::value>, dim3(groups(count, kMany)), kThreads, 0, stream,
             static_cast<const typename T::elem*>(x), x_stride, codes, scales, count, (uint32_t)(k / kLane));
     });
     return hip_status("nqx_quantize", e);
@@ -171,7 +222,7 @@ extern "C" int nqx_dequantize(const uint8_t* codes, const uint8_t* scales, void*
     by_type(dtype, format, [&](auto t, auto f) {
         using T = decltype(t);
         const int64_t count = rows * (k / kLane);
-        e = start(&mx_dequantize_kernel<T, decltype(f)::value>, dim3(grid_for(count)), kThreads, 0, static_cast<hipStream_t>(stream), 
+        e = start(&mx_dequantize_kernel<T, decltype(f)::value>, dim3(groups(count, kMany)), kThreads, 0, static_cast<hipStream_t>(stream),
             codes, scales, static_cast<typename T::elem*>(y), count);
     });
     return hip_status("nqx_dequantize", e);
@@ -183,7 +234,7 @@ extern "C" int nqx_add_rmsnorm(const void* x, int64_t x_stride, const void* delt
     const char* fn = "nqx_add_rmsnorm";
     if (int s = check_types(fn, rows, k, dtype, format)) return s;
     if (k > 16384) return refuse(NQX_ERR_UNSUPPORTED, "%s: k must be at most 16384, got %lld", fn, (long long)k);
-    if (rows >= ((int64_t)1 << 31)) return refuse(NQX_ERR_UNSUPPORTED, "%s: too many rows (%lld)", fn, (long long)rows);
+    if (rows >= ((int64_t)1 << 24)) return refuse(NQX_ERR_UNSUPPORTED, "%s: fewer than 2^24 rows at a time, got %lld", fn, (long long)rows);
     if (rows == 0) return NQX_OK;
     if (int s = check_rows(fn, "x", x, x_stride, k, dtype)) return s;
     if (delta) {
@@ -202,13 +253,14 @@ extern "C" int nqx_add_rmsnorm(const void* x, int64_t x_stride, const void* delt
         using T = decltype(t);
         using E = typename T::elem;
         const auto with = [&](auto chunks) {
-            e = start(&mx_add_rmsnorm_kernel<T, decltype(f)::value, decltype(chunks)::value>, dim3((unsigned)rows), kThreads, 0, static_cast<hipStream_t>(stream), 
+            e = start(&mx_add_rmsnorm_kernel<T, decltype(f)::value, decltype(chunks)::value>, dim3((unsigned)rows), kThreads, 0, static_cast<hipStream_t>(stream),
                     static_cast<const E*>(x), x_stride, static_cast<const E*>(delta), delta_stride, static_cast<const E*>(weight),
                     static_cast<E*>(total), codes, scales, (uint32_t)(k / kLane), eps);
         };
         const int64_t chunks = cdiv(k / kLane, kThreads);
         if (chunks <= 1) with(Const<1>());
         else if (chunks <= 2) with(Const<2>());
+        else if (chunks <= 3) with(Const<3>());
         else if (chunks <= 4) with(Const<4>());
         else with(Const<8>());
     });
@@ -228,7 +280,7 @@ extern "C" int nqx_silu_mul(const void* gate, int64_t gate_stride, const void* u
         using T = decltype(t);
         using E = typename T::elem;
         const int64_t count = rows * (k / kLane);
-        e = start(&mx_silu_mul_kernel<T, decltype(f)::value>, dim3(grid_for(count)), kThreads, 0, static_cast<hipStream_t>(stream), 
+        e = start(&mx_silu_mul_kernel<T, decltype(f)::value>, dim3(groups(count, 2)), kThreads, 0, static_cast<hipStream_t>(stream),
             static_cast<const E*>(gate), gate_stride, static_cast<const E*>(up), up_stride, codes, scales, count,
             (uint32_t)(k / kLane));
     });

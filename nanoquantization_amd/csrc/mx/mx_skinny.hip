@@ -55,10 +55,11 @@ __global__ __launch_bounds__(kThreads) void mx_skinny_kernel(const void* __restr
         const int per_row = steps * 16;              // eights
         for (int i = threadIdx.x; i < (int)rows * per_row; i += kThreads) {
             const int r = i / per_row, e = i - r * per_row;
-            float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-            if (e < blocks * 4) load8<T>(static_cast<const E*>(x) + r * x_stride + e * 8, v);
-            const uint32_t byte = scale_byte<FORMAT>(max_of_block(magnitude_bits(v)));
-            const u32x2 code = encode8<FORMAT>(v, byte);
+            Eight<T, FORMAT> v;
+            v.clear();
+            if (e < blocks * 4) v.load(static_cast<const E*>(x) + r * x_stride + e * 8);
+            uint32_t byte;
+            const u32x2 code = v.encode(byte);
             if constexpr (kFour) *reinterpret_cast<uint32_t*>(s_x + r * r_bytes + e * 4) = code.x;
             else *reinterpret_cast<u32x2*>(s_x + r * r_bytes + e * 8) = code;
             if ((e & 3) == 0) s_x[(int)rows * r_bytes + r * steps * 4 + (e >> 2)] = (unsigned char)byte;

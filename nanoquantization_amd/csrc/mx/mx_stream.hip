@@ -38,22 +38,6 @@ int splits_of(int64_t rows, int64_t n, int64_t k) {
     if (s > 16) s = 16;
     return s < 1 ? 1 : (int)s;
 }
-// Weight rows of a workgroup, and splits of k: as many as fill the chip with workgroups that are resident at once, of a group of
-// chunks each at least.  With 33 to 64 rows of x 256 weight rows share them, unless 128 do without a split, whose sums would cost
-// another launch.
-struct Plan {
-    int weight_rows, splits;
-};
-Plan plan_of(int64_t rows, int64_t n, int64_t k) {
-    const int mt = sixteens(rows), per = group_chunks(mt);
-    const int64_t blocks = k / kBlock, groups = (blocks & 7 ? 1 : 0) + ((blocks >> 3) + per - 1) / per, most = 256 * per_cu(mt);
-    const int wide = mt == 4 && (cdiv(n, 256) >= 160 || cdiv(n, 128) < 160) ? 256 : 128;
-    int64_t s = cdiv(n, wide) >= 160 ? 1 : most / cdiv(n, wide);
-    if (s > groups) s = groups;
-    if (s > 16) s = 16;
-    return {wide, s < 1 ? 1 : (int)s};
-}
-
 template <int FORMAT, int MT, bool RAW>
 struct Stream {
     static constexpr int kFours = fours(MT), kWaves = 4 * kFours, kThreads = 64 * kWaves, kBufs = 3, kGroup = group_chunks(MT), kBytes = 8 * kGroup;     // kBytes: a row's scales of a group
@@ -219,10 +203,11 @@ __global__ __launch_bounds__(256 * fours(MT)) void mx_stream_kernel(const void* 
         for (int r = 0; r < rows; ++r)
             for (int e = threadIdx.x; e < per_row; e += kThreads) {
                 const int c = c0 + (e >> 5), in_chunk = (e & 31) * 8, at = 256 * (c < first ? whole : c - first) + in_chunk;
-                float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-                if (at < blocks * 32) load8<T>(static_cast<const E*>(x) + r * x_stride + at, v);
-                const uint32_t byte = scale_byte<FORMAT>(max_of_block(magnitude_bits(v)));
-                const u32x2 code = encode8<FORMAT>(v, byte);
+                Eight<T, FORMAT> v;
+                v.clear();
+                if (at < blocks * 32) v.load(static_cast<const E*>(x) + r * x_stride + at);
+                uint32_t byte;
+                const u32x2 code = v.encode(byte);
                 const int b = in_chunk >> 5, within = in_chunk & 31;               // block of the chunk
                 if constexpr (kFour) {
                     *reinterpret_cast<uint32_t*>(s_x + r * r_bytes + (c - c0) * 128 + swizzle(r, b) * 16 + within / 2) = code.x;
@@ -342,8 +327,9 @@ __global__ __launch_bounds__(256 * fours(MT)) void mx_stream_kernel(const void* 
 template <typename T>
 __global__ __launch_bounds__(256) void mx_add_splits_kernel(const float* __restrict__ sums, const typename T::elem* __restrict__ bias,
                                                             typename T::elem* __restrict__ y, int rows, int N, int pitch, int splits) {
-    const int64_t at = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4, n = at % pitch, m = at / pitch;
-    if (m >= rows || n >= N) return;
+    // fewer than 160 tiles of 128 x 128 sums: 32 bits
+    const uint32_t at = (blockIdx.x * 256 + threadIdx.x) * 4, m = at / (uint32_t)pitch, n = at - m * pitch;
+    if (m >= (uint32_t)rows || n >= (uint32_t)N) return;
     f32x4 v = *reinterpret_cast<const f32x4*>(sums + at);
     for (int s = 1; s < splits; s += 4) {            // four on their way at once
         f32x4 next[4];

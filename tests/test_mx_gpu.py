@@ -487,3 +487,117 @@ def test_past_32_bits():
         assert torch.equal(y[r:r + 1], nq.mx_linear(x[r:r + 1].clone(), w, ws))
     del y
     torch.cuda.empty_cache()
+
+
+# ---- where one kernel hands over to another -------------------------------------------------------------------------------
+def _form(rows, n, k, fmt, quantised=1):
+    return _lib.mx_lib().nqx_linear_form(rows, n, k, 1, FORMATS.index(fmt), quantised).decode()
+
+
+# tiles of 128 and of 256: k of less than a chunk of 256, of whole ones, of both, of four and more; rows of scales of whole words or not
+TILES = [(2100, 32, 2100), (2177, 96, 2049), (2049, 256, 2100), (2100, 288, 2177), (2180, 544, 2061), (2051, 1024, 2176), (2100, 1120, 2055),
+         (2050, 2528, 2100), (2900, 32, 4096), (2817, 224, 4095), (3300, 512, 3890), (3330, 768, 3841), (2900, 1184, 4097), (2818, 2080, 4100)]
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("rows,k,n", TILES)
+def test_tiles(rows, k, n, fmt):
+    assert _form(rows, n, k, fmt) == "mx_tiles_kernel " + ("128 x 128" if rows < 2200 else "256 x 256")
+    dtype = (torch.bfloat16, torch.float16, torch.float32)[(rows + n + k // 32) % 3]
+    w, ws = _weight(n, n, k)
+    codes, scales = nq.mx_quantize(_random(rows, rows, k, dtype=torch.float32), fmt)
+    bias = _random(k, n, dtype=dtype, spread=False) if (rows + k // 32) % 2 else None
+    y = nq.mx_linear_quantized(codes, scales, w, ws, bias, dtype)
+    _check_product(y, (codes, scales), (w, ws), bias, dtype)
+    # scales at any address
+    ws_off, scales_off = (torch.empty(t.numel() + 1, dtype=torch.uint8, device="cuda")[1:].view_as(t).copy_(t) for t in (ws, scales))
+    assert torch.equal(nq.mx_linear_quantized(codes, scales_off, w, ws, bias, dtype), y)
+    assert torch.equal(nq.mx_linear_quantized(codes, scales, w, ws_off, bias, dtype), y)
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("rows,k,n", [(2100, 1184, 2100), (2900, 1184, 4096), (2900, 1024, 4096)])
+def test_tiles_of_every_code(rows, k, n, fmt):
+    g = _gen(rows + k)
+    w = torch.randint(0, 256, (n, k // 2), device="cuda", generator=g, dtype=torch.uint8)
+    ws = torch.randint(100, 150, (n, k // 32), device="cuda", generator=g, dtype=torch.uint8)
+    codes = torch.randint(0, 256, (rows, k // (2 if fmt == "mxfp4" else 1)), device="cuda", generator=g, dtype=torch.uint8)
+    if fmt == "mxfp8":
+        codes = torch.where(codes % 128 == 127, codes - 1, codes)           # without the two NaN codes
+    scales = torch.randint(100, 150, (rows, k // 32), device="cuda", generator=g, dtype=torch.uint8)
+    _check_product(nq.mx_linear_quantized(codes, scales, w, ws, None, torch.float32), (codes, scales), (w, ws), None, torch.float32)
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("rows,k,n", [(2100, 1120, 2100), (2900, 1120, 4100)])
+def test_nan_stays_in_its_rows_of_tiles(rows, k, n, fmt):
+    w, ws = _weight(5, n, k)
+    codes, scales = nq.mx_quantize(_random(6, rows, k), fmt)
+    clean = nq.mx_linear_quantized(codes, scales, w, ws)
+    for block in (0, 17, k // 32 - 1):
+        bad = scales.clone()
+        bad[rows - 1, block] = 255
+        y = nq.mx_linear_quantized(codes, bad, w, ws)
+        assert torch.isnan(y[rows - 1]).all() and torch.equal(y[:rows - 1], clean[:rows - 1])
+        bad = ws.clone()
+        bad[n - 1, block] = 255
+        y = nq.mx_linear_quantized(codes, scales, w, bad)
+        assert torch.isnan(y[:, n - 1]).all() and torch.equal(y[:, :n - 1], clean[:, :n - 1])
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("rows,k,n", [(1, 1024, 65536), (1, 1056, 65536), (4, 4096, 2048), (5, 4096, 2048), (16, 2048, 4096), (16, 2080, 4096), (17, 2048, 1024),
+                                      (32, 1184, 1100), (33, 4128, 200), (64, 2336, 130), (65, 4096, 130), (128, 4128, 129), (129, 4096, 127)])
+def test_around_the_borders(rows, k, n, fmt):
+    """Of x as it is and quantised before, scales at any address: the same bits where one kernel runs them."""
+    w, ws = _weight(n, n, k)
+    x, bias = _random(rows, rows, k), _random(k, n, spread=False)
+    codes, scales = nq.mx_quantize(x, fmt)
+    y = nq.mx_linear_quantized(codes, scales, w, ws, bias)
+    if rows * n * k < 1 << 28:
+        _check_product(y, (codes, scales), (w, ws), bias, torch.bfloat16)
+    ws_off, scales_off = (torch.empty(t.numel() + 1, dtype=torch.uint8, device="cuda")[1:].view_as(t).copy_(t) for t in (ws, scales))
+    assert torch.equal(nq.mx_linear_quantized(codes, scales_off, w, ws_off, bias), y)
+    assert torch.equal(nq.mx_linear(x, w, ws, bias, fmt), y) and torch.equal(nq.mx_linear(x, w, ws_off, bias, fmt), y)
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("rows", [1, 20])
+def test_a_row_longer_than_a_buffer_reaches(rows, fmt):
+    k, n = (1 << 22) + 96, 3
+    w, ws = _weight(4, n, k)
+    x = _random(5, rows, k)
+    codes, scales = nq.mx_quantize(x, fmt)
+    y = nq.mx_linear(x, w, ws, activations=fmt)
+    _check_product(y, (codes, scales), (w, ws), None, torch.bfloat16)
+    assert torch.equal(y, nq.mx_linear_quantized(codes, scales, w, ws))
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+def test_two_streams_at_once(fmt):
+    """Products whose sums meet in a workspace, and row kernels, of two streams that overlap."""
+    w, ws = _weight(1, 512, 9728)
+    xs = [_random(i, 40, 9728) for i in range(2)]
+    want = [nq.mx_linear(x, w, ws, activations=fmt) for x in xs]
+    streams = [torch.cuda.Stream() for _ in xs]
+    torch.cuda.synchronize()
+    got = [[], []]
+    for _ in range(20):
+        for i, st in enumerate(streams):
+            with torch.cuda.stream(st):
+                got[i].append(nq.mx_linear(xs[i], w, ws, activations=fmt))
+    torch.cuda.synchronize()
+    assert all(torch.equal(y, want[i]) for i in range(2) for y in got[i])
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+def test_silu_of_every_gate(fmt):
+    """Gates close together from where the exponential overflows to where it vanishes; up large enough that small results count."""
+    steps = torch.linspace(-110, 110, 8192, device="cuda")
+    gate = steps.unsqueeze(1).expand(-1, 32).contiguous()
+    for factor in (1.0, 2.0 ** 40):
+        up = torch.full_like(gate, factor)
+        g = gate.cpu().double()
+        want = g * torch.sigmoid(g) * factor
+        # below 2^-125 the reciprocal may be zero
+        _check_rounded(nq.mx_silu_mul(gate, up, fmt), want, fmt, 12 * U, 110 * 2.0 ** -125 * factor)

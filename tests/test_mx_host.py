@@ -184,3 +184,14 @@ def test_oracle_scales():
     assert byte(448.0, "mxfp8") == byte(464.0, "mxfp8") == 127 and byte(464.0 + 2.0 ** -30, "mxfp8") == 128
     assert byte(0.0, "mxfp4") == byte(2.0 ** -149, "mxfp8") == 0
     assert byte(float("inf"), "mxfp4") == byte(float("nan"), "mxfp8") == 255
+
+
+def test_sizes_past_a_launch_are_refused():
+    """2^36 values and more, 2^24 rows of a norm, weights of more than 2^29 rows: refused before a pointer is looked at."""
+    L, at = _lib.mx_lib(), 4096
+    assert L.nqx_quantize(at, 1 << 16, at, at, 1 << 20, 1 << 16, 1, 0, None) == 2 and b"too large" in L.nqx_last_error()
+    assert L.nqx_dequantize(at, at, at, 1 << 31, 32, 1, 0, None) == 2
+    assert L.nqx_silu_mul(at, 1 << 16, at, 1 << 16, at, at, 1 << 20, 1 << 16, 1, 0, None) == 2
+    assert L.nqx_add_rmsnorm(at, 32, None, 0, at, None, at, at, 1 << 24, 32, 1e-6, 1, 0, None) == 2 and b"2^24" in L.nqx_last_error()
+    assert L.nqx_linear_workspace_bytes(1, (1 << 29) + 1, 32, 1, 0, 0) == 0
+    assert L.nqx_linear(at, 32, at, at, None, at, 1, (1 << 29) + 1, 32, 1, 0, None, 0, None) == 2
