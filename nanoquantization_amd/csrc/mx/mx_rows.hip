@@ -1,7 +1,7 @@
 // Row kernels of the microscaled formats: quantise, dequantise, residual addition + RMSNorm, SiLU(gate) * up.  All are
 // bound by memory: a lane takes eight consecutive values in one or two 16-byte loads, several eights at once, the four lanes of
 // a block agree on the largest magnitude by two DPP moves, and codes leave in 4- or 8-byte stores, whole lines a wave.  In bf16,
-// 25600 x 5120: quantise to e2m1 68 us (4.9 TB/s; 88 to e4m3, 4.5), dequantise 53 and 58 (6.3 and 6.8 with the codes still in
+// 25600 x 5120: quantise to e2m1 67 us (5.0 TB/s; 88 to e4m3, 4.5), dequantise 53 and 58 (6.3 and 6.8 with the codes still in
 // the last cache); 8192 x 5120: sum, norm and e4m3 63 us (4.7 TB/s).  A large copy reaches 5.2.
 #include "mx_common.hpp"
 
@@ -14,27 +14,37 @@ constexpr int kThreads = 256;
 constexpr int kMany = 4;
 
 // Where eight `at` of rows `stride` values apart begins.  Dense rows need no division, which would cost a launch of a few rows a
-// microsecond.
-__device__ __forceinline__ int64_t place(int64_t at, int64_t stride, uint32_t per_row) {
-    if (stride == (int64_t)per_row * 8) return at * 8;
-    if ((at >> 32) == 0) {
-        const uint32_t row = (uint32_t)at / per_row;
-        return row * stride + (int64_t)((uint32_t)at - row * per_row) * 8;
+// microsecond; others, of fewer than 2^31 eights, one by a product: with 2^(bits - 1) < per_row <= 2^bits and magic =
+// 2^(31 + bits) / per_row rounded up, at * magic / 2^(31 + bits) is past at / per_row by less than 1 / per_row.
+struct Rows {
+    uint32_t per_row, magic, bits;           // magic 0: 2^31 eights or more
+};
+Rows rows_of(int64_t count, int64_t k) {
+    Rows r = {(uint32_t)(k / kLane), 0, 0};
+    while ((1u << r.bits) < r.per_row) ++r.bits;
+    if (count < ((int64_t)1 << 31)) r.magic = (uint32_t)((((uint64_t)1 << (31 + r.bits)) + r.per_row - 1) / r.per_row);
+    return r;
+}
+__device__ __forceinline__ int64_t place(int64_t at, int64_t stride, Rows r) {
+    if (stride == (int64_t)r.per_row * 8) return at * 8;
+    if (r.magic) {
+        const uint32_t row = __umulhi((uint32_t)at, r.magic) >> (r.bits - 1);
+        return row * stride + (int64_t)((uint32_t)at - row * r.per_row) * 8;
     }
-    const int64_t row = at / per_row;
-    return row * stride + (at - row * per_row) * 8;
+    const int64_t row = at / r.per_row;
+    return row * stride + (at - row * r.per_row) * 8;
 }
 
 template <typename T, int FORMAT>
 __global__ __launch_bounds__(kThreads) void mx_quantize_kernel(const typename T::elem* __restrict__ x, int64_t stride,
                                                                uint8_t* __restrict__ codes, uint8_t* __restrict__ scales,
-                                                               int64_t count, uint32_t per_row) {
+                                                               int64_t count, Rows in) {
     const int64_t first = (int64_t)blockIdx.x * (kMany * kThreads) + threadIdx.x;
     Eight<T, FORMAT> e[kMany];
 #pragma unroll
     for (int u = 0; u < kMany; ++u) {
         const int64_t at = first + u * kThreads;
-        if (at < count) e[u].load(x + place(at, stride, per_row));
+        if (at < count) e[u].load(x + place(at, stride, in));
     }
 #pragma unroll
     for (int u = 0; u < kMany; ++u) {
@@ -144,10 +154,10 @@ __global__ __launch_bounds__(kThreads) void mx_add_rmsnorm_kernel(const typename
 // gate / (1 + exp(-gate)) * up.  exp(-g) is 2^t 2^r, t = -g log2(e) rounded and r what that and the constant lost: without r the
 // relative error grows with |g|.  (2^r as a factor of its own near 1: where 2^t is infinite a sum could be inf - inf.)  The
 // reciprocal is off by a step of fp32 at most, a division would be by half of one and takes ten times as long (8192 x 12288 bf16
-// to e2m1 is 104 us, 4.4 TB/s, and was 116 with expf and a division).  Past 100 the exponential is infinite or does not change 1.
+// to e2m1 is 102 us, 4.5 TB/s, and was 116 with expf and a division).  Past 100 the exponential is infinite or does not change 1.
 __device__ __forceinline__ float silu_mul(float gate, float up) {
     constexpr float kHigh = 1.44269502f, kLow = 1.92596303e-8f, kLn2 = 0.693147182f;
-    const float g = -fminf(fmaxf(gate, -100.f), 100.f), t = g * kHigh;
+    const float g = -__builtin_amdgcn_fmed3f(gate, -100.f, 100.f), t = g * kHigh;
     const float r = __builtin_fmaf(g, kLow, __builtin_fmaf(g, kHigh, -t));
     const float e = __builtin_amdgcn_exp2f(t) * __builtin_fmaf(r, kLn2, 1.0f);
     return gate * __builtin_amdgcn_rcpf(1.0f + e) * up;
@@ -157,14 +167,14 @@ template <typename T, int FORMAT>
 __global__ __launch_bounds__(kThreads) void mx_silu_mul_kernel(const typename T::elem* __restrict__ gate, int64_t gate_stride,
                                                                const typename T::elem* __restrict__ up, int64_t up_stride,
                                                                uint8_t* __restrict__ codes, uint8_t* __restrict__ scales,
-                                                               int64_t count, uint32_t per_row) {
+                                                               int64_t count, Rows in) {
     constexpr int kTwo = 2;                  // eights of a lane: they are two loads each
     const int64_t first = (int64_t)blockIdx.x * (kTwo * kThreads) + threadIdx.x;
     Eight<T, FORMAT> g[kTwo], u[kTwo];
 #pragma unroll
     for (int i = 0; i < kTwo; ++i) {
         const int64_t at = first + i * kThreads;
-        if (at < count) g[i].load(gate + place(at, gate_stride, per_row)), u[i].load(up + place(at, up_stride, per_row));
+        if (at < count) g[i].load(gate + place(at, gate_stride, in)), u[i].load(up + place(at, up_stride, in));
     }
 #pragma unroll
     for (int i = 0; i < kTwo; ++i) {
@@ -189,7 +199,7 @@ int quantize(const void* x, int64_t x_stride, uint8_t* codes, uint8_t* scales, i
         using T = decltype(t);
         const int64_t count = rows * (k / kLane);
         e = start(&mx_quantize_kernel<T, decltype(f)::value>, dim3(groups(count, kMany)), kThreads, 0, stream,
-            static_cast<const typename T::elem*>(x), x_stride, codes, scales, count, (uint32_t)(k / kLane));
+            static_cast<const typename T::elem*>(x), x_stride, codes, scales, count, rows_of(count, k));
     });
     return hip_status("nqx_quantize", e);
 }
@@ -282,7 +292,7 @@ extern "C" int nqx_silu_mul(const void* gate, int64_t gate_stride, const void* u
         const int64_t count = rows * (k / kLane);
         e = start(&mx_silu_mul_kernel<T, decltype(f)::value>, dim3(groups(count, 2)), kThreads, 0, static_cast<hipStream_t>(stream),
             static_cast<const E*>(gate), gate_stride, static_cast<const E*>(up), up_stride, codes, scales, count,
-            (uint32_t)(k / kLane));
+            rows_of(count, k));
     });
     return hip_status(fn, e);
 }

@@ -601,3 +601,25 @@ def test_silu_of_every_gate(fmt):
         want = g * torch.sigmoid(g) * factor
         # below 2^-125 the reciprocal may be zero
         _check_rounded(nq.mx_silu_mul(gate, up, fmt), want, fmt, 12 * U, 110 * 2.0 ** -125 * factor)
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("rows,k", [(4099, 32), (3001, 96), (1021, 224), (517, 1056), (9, 25568), (2, 4064)])
+def test_rows_apart(rows, k, fmt):
+    """Row kernels of rows that are not next to each other, of sizes that no power of two divides."""
+    wide = _random(rows, rows, 2 * k + 8)
+    a, b = wide[:, :k], wide[:, k + 8:]
+    for got, want in ((nq.mx_quantize(b, fmt), nq.mx_quantize(b.contiguous(), fmt)),
+                      (nq.mx_silu_mul(a, b, fmt), nq.mx_silu_mul(a.contiguous(), b.contiguous(), fmt))):
+        assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+
+
+def test_more_eights_than_31_bits():
+    base = _random(1, 1, 32)
+    x = base.expand((1 << 29) + 3, 32)
+    codes, scales = nq.mx_quantize(x, "mxfp4")
+    one = nq.mx_quantize(base, "mxfp4")
+    assert torch.equal(codes[-9:], one[0].expand(9, 16)) and torch.equal(codes[::1 << 21], one[0].expand(257, 16))
+    assert bool((scales == one[1]).all())
+    del x, codes, scales
+    torch.cuda.empty_cache()
