@@ -64,14 +64,19 @@ __global__ __launch_bounds__(256 * fours(MT)) void mx_stream_kernel(const void* 
                                                         const uint8_t* __restrict__ w, const uint8_t* __restrict__ ws,
                                                         const typename T::elem* __restrict__ bias, typename T::elem* __restrict__ y,
                                                         float* __restrict__ sums, int rows, int N, int blocks, int words, int groups_each,
-                                                        int groups_more) {
+                                                        int groups_more, uint32_t row_tiles) {
     using G = Stream<FORMAT, MT, RAW>;
     constexpr bool kFour = FORMAT == NQX_FP4;
     constexpr int kWaves = G::kWaves, kThreads = G::kThreads, kWT = G::kWT, kXT = G::kXT, kGroup = G::kGroup, kBytes = G::kBytes;
     extern __shared__ __attribute__((aligned(16))) unsigned char s_mem[];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lo = lane & 15, hi = lane >> 4;
-    const int split = blockIdx.y, n0 = blockIdx.x * kRows;
-    const int n_rows = N - n0 < kRows ? N - n0 : kRows, m0 = blockIdx.z * (16 * MT), all_rows = rows;
+    // The row tiles of a weight tile run next to each other on one XCD (workgroups go round the eight of them), whose L2 then has
+    // the weight for all but the first: 333 rows by 2816 x 9728 in 8 bits 18.8 us, 19.1 across
+    // XCDs; 1000 by 4096 x 4096 25.1 and 27.1.
+    const uint32_t turn = blockIdx.x >> 3, tile = row_tiles == 1 ? blockIdx.x : turn / row_tiles * 8 + (blockIdx.x & 7);
+    const int split = blockIdx.y, n0 = (int)(tile * kRows), m0 = row_tiles == 1 ? 0 : (int)(turn % row_tiles) * (16 * MT);
+    if (n0 >= N) return;
+    const int n_rows = N - n0 < kRows ? N - n0 : kRows, all_rows = rows;
     rows = rows - m0 < 16 * MT ? rows - m0 : 16 * MT;
     const uint32_t w_pitch = (uint32_t)blocks * 16, x_pitch = (uint32_t)blocks * (kFour ? 16 : 32);
     // Chunks: the blocks that do not fill one come first (pieces that do not exist are asked for past the buffer's end, which
@@ -311,7 +316,7 @@ __global__ __launch_bounds__(256 * fours(MT)) void mx_stream_kernel(const void* 
 #pragma unroll
             for (int i = 0; i < kWT; ++i) acc[i][j] += meet[(j * kWT + i) * 64];
     }
-    const int64_t pitch = (int64_t)gridDim.x * kRows;
+    const int64_t pitch = ((int64_t)N + kRows - 1) / kRows * kRows;
 #pragma unroll
     for (int j = 0; j < kXT; ++j)
 #pragma unroll
@@ -358,9 +363,10 @@ hipError_t launch(const Product& p, hipStream_t stream) {
     const E *bias = static_cast<const E*>(p.bias);
     E* y = static_cast<E*>(p.y);
     const int groups = (blocks & 7 ? 1 : 0) + ((blocks >> 3) + G::kGroup - 1) / G::kGroup;
-    const hipError_t e = start(&mx_stream_kernel<T, FORMAT, MT, RAW>, dim3(tiles, splits, (unsigned)cdiv(p.rows, 16 * MT)), G::kThreads, lds, stream, RAW ? p.raw : p.x,
-                               p.raw_stride, p.xs, p.w, p.ws, bias, y, p.sums, (int)p.rows, (int)p.n, blocks, words, groups / splits,
-                               groups % splits);
+    const unsigned row_tiles = (unsigned)cdiv(p.rows, 16 * MT);
+    const dim3 grid(row_tiles == 1 ? tiles : cdiv(tiles, 8) * 8 * row_tiles, splits);
+    const hipError_t e = start(&mx_stream_kernel<T, FORMAT, MT, RAW>, grid, G::kThreads, lds, stream, RAW ? p.raw : p.x, p.raw_stride, p.xs,
+                               p.w, p.ws, bias, y, p.sums, (int)p.rows, (int)p.n, blocks, words, groups / splits, groups % splits, row_tiles);
     if (e != hipSuccess || splits == 1) return e;
     const int pitch = tiles * kRows;
     return start(&mx_add_splits_kernel<T>, dim3((unsigned)cdiv(p.rows * pitch, 1024)), 256, 0, stream, p.sums, bias, y, (int)p.rows, (int)p.n,
