@@ -39,28 +39,36 @@ __device__ __forceinline__ f32x16 mfma32(u32x4 w, u32x4 x, f32x16 c, uint32_t w_
     return __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(a, b, c, 4, 4, BYTE, (int)w_scale, BYTE, (int)x_scale);
 }
 
-// Four consecutive values of a row of y, columns n .. n + 3 of which those below N exist.
-template <typename T>
-__device__ __forceinline__ void store_sums(f32x4 v, typename T::elem* y, const typename T::elem* bias, int64_t row, int64_t n,
+// 4 Q consecutive values of a row of y, columns n and on, of which those below N exist.
+template <typename T, int Q>
+__device__ __forceinline__ void store_sums(f32x4 (&v)[Q], typename T::elem* y, const typename T::elem* bias, int64_t row, int64_t n,
                                            int64_t N) {
     typename T::elem* to = y + row * N + n;
-    if (n + 4 <= N) {
-        if (bias) {
+    if (bias) {
 #pragma unroll
-            for (int r = 0; r < 4; ++r) v[r] += T::to_f32(bias[n + r]);
-        }
+        for (int r = 0; r < 4 * Q; ++r) v[r / 4][r % 4] += T::to_f32(bias[n + r < N ? n + r : N - 1]);
+    }
+    if (n + 4 * Q <= N) {
         // any address of the type
         if constexpr (sizeof(typename T::elem) == 4) {
-            __builtin_memcpy(to, &v, 16);
+            __builtin_memcpy(to, v, 16 * Q);
         } else {
-            const u32x2 w = {T::pack2(v[0], v[1]), T::pack2(v[2], v[3])};
-            __builtin_memcpy(to, &w, 8);
+            uint32_t w[2 * Q];
+#pragma unroll
+            for (int q = 0; q < Q; ++q) w[2 * q] = T::pack2(v[q][0], v[q][1]), w[2 * q + 1] = T::pack2(v[q][2], v[q][3]);
+            __builtin_memcpy(to, w, 8 * Q);
         }
         return;
     }
 #pragma unroll
-    for (int r = 0; r < 3; ++r)
-        if (n + r < N) to[r] = T::from_f32(bias ? v[r] + T::to_f32(bias[n + r]) : v[r]);
+    for (int r = 0; r < 4 * Q - 1; ++r)
+        if (n + r < N) to[r] = T::from_f32(v[r / 4][r % 4]);
+}
+template <typename T>
+__device__ __forceinline__ void store_sums(f32x4 v, typename T::elem* y, const typename T::elem* bias, int64_t row, int64_t n,
+                                           int64_t N) {
+    f32x4 one[1] = {v};
+    store_sums<T, 1>(one, y, bias, row, n, N);
 }
 
 int skinny_product(const Product& p, hipStream_t stream);       // at most 16 rows of raw x

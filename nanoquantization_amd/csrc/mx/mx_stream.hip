@@ -50,8 +50,8 @@ struct Stream {
     static constexpr int kNone = kXAt + kBufs * kX;                         // where a wave without a piece of x lets its request go
     static constexpr int kScales = kNone + (kXAll % kWaves ? 1024 : 0), kSlot = (kRows + (RAW ? 0 : 16 * MT)) * kBytes;
     static constexpr int kFixed = kScales + 2 * kSlot;
-    static constexpr int kMeet = kFours == 2 ? 4 * kWT * kXT * 1024 : 0;      // bytes of LDS where the two fours' sums meet, in the buffers' place
-    static_assert(kMeet <= kNone, "");
+    static constexpr int kSumPitch = kRows + 4;      // floats of a row of sums of two fours, in the buffers' place
+    static_assert(kFours == 1 || 16 * MT * kSumPitch * 4 <= kNone, "");
     static_assert(kFixed * per_cu(MT) <= 160 * 1024 , "");
 };
 // RAW: bytes of `rows` quantised rows of `chunks` chunks in LDS, codes and scales.
@@ -71,8 +71,8 @@ __global__ __launch_bounds__(256 * fours(MT)) void mx_stream_kernel(const void* 
     extern __shared__ __attribute__((aligned(16))) unsigned char s_mem[];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lo = lane & 15, hi = lane >> 4;
     // The row tiles of a weight tile run next to each other on one XCD (workgroups go round the eight of them), whose L2 then has
-    // the weight for all but the first: 333 rows by 2816 x 9728 in 8 bits 18.8 us, 19.1 across
-    // XCDs; 1000 by 4096 x 4096 25.1 and 27.1.
+    // the weight for all but the first: 333 rows by 2816 x 9728 in 8 bits 17.8 us, 18.1 across
+    // XCDs; 1000 by 4096 x 4096 24.5 and 26.5.
     const uint32_t turn = blockIdx.x >> 3, tile = row_tiles == 1 ? blockIdx.x : turn / row_tiles * 8 + (blockIdx.x & 7);
     const int split = blockIdx.y, n0 = (int)(tile * kRows), m0 = row_tiles == 1 ? 0 : (int)(turn % row_tiles) * (16 * MT);
     if (n0 >= N) return;
@@ -300,23 +300,49 @@ __global__ __launch_bounds__(256 * fours(MT)) void mx_stream_kernel(const void* 
 #pragma unroll 1
     for (; c < c1; ++c) chunk(Const<0>(), c);
     __builtin_amdgcn_s_waitcnt(0x0F70);              // vmcnt(0): no request is on its way to LDS that is another workgroup's by then
+    const int64_t pitch = ((int64_t)N + kRows - 1) / kRows * kRows;          // of a row of sums
     if constexpr (G::kFours == 2) {
+        // The two fours' sums meet in LDS, and leave it row by row, 16 bytes a lane.  (Straight from the registers of one four a
+        // store has 32 bytes of each of 16 rows: 333 rows by 2816 x 9727 took 20.7 us, and 18.1 so.)
+        using E = typename T::elem;
+        float* s_sum = reinterpret_cast<float*>(s_mem);
+        const auto at = [&](int i, int j) {
+            return reinterpret_cast<f32x4*>(s_sum + (x_row + 16 * j) * G::kSumPitch + wm * (16 * kWT) + 16 * i + 4 * hi);
+        };
         __syncthreads();
-        f32x4* meet = reinterpret_cast<f32x4*>(s_mem) + own * (kWT * kXT * 64) + lane;
         if (mine == 1) {
 #pragma unroll
             for (int j = 0; j < kXT; ++j)
 #pragma unroll
-                for (int i = 0; i < kWT; ++i) meet[(j * kWT + i) * 64] = acc[i][j];
+                for (int i = 0; i < kWT; ++i) *at(i, j) = acc[i][j];
         }
         __syncthreads();
-        if (mine == 1) return;
+        if (mine == 0) {
 #pragma unroll
-        for (int j = 0; j < kXT; ++j)
+            for (int j = 0; j < kXT; ++j)
 #pragma unroll
-            for (int i = 0; i < kWT; ++i) acc[i][j] += meet[(j * kWT + i) * 64];
+                for (int i = 0; i < kWT; ++i) *at(i, j) += acc[i][j];
+        }
+        __syncthreads();
+        const auto rows_out = [&](auto v_, auto put) {
+            constexpr int V = decltype(v_)::value, kOf = kRows / V;          // values of a lane, lanes of a row
+            for (int e = threadIdx.x; e < rows * kOf; e += kThreads) {
+                const int r = e / kOf, c = e % kOf * V;
+                f32x4 v[V / 4];
+#pragma unroll
+                for (int q = 0; q < V / 4; ++q) v[q] = *reinterpret_cast<const f32x4*>(s_sum + r * G::kSumPitch + c + 4 * q);
+                if (n0 + c < N) put(v, m0 + r, n0 + c);
+            }
+        };
+        if (gridDim.y > 1) {
+            rows_out(Const<4>(), [&](f32x4 (&v)[1], int m, int n) {
+                *reinterpret_cast<f32x4*>(sums + ((int64_t)split * all_rows + m) * pitch + n) = v[0];
+            });
+        } else {
+            rows_out(Const<16 / sizeof(E)>(), [&](auto& v, int m, int n) { store_sums<T>(v, y, bias, m, n, N); });
+        }
+        return;
     }
-    const int64_t pitch = ((int64_t)N + kRows - 1) / kRows * kRows;
 #pragma unroll
     for (int j = 0; j < kXT; ++j)
 #pragma unroll
