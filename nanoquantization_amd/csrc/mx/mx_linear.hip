@@ -31,11 +31,14 @@ Form form_of(int64_t rows, int64_t n, int64_t k) {
     if (rows <= 128 || cdiv(rows, 128) * cdiv(n, 128) <= 256) return kStream;
     return cdiv(rows, 256) * cdiv(n, 256) >= 192 ? kTiles256 : kTiles128;
 }
-// Whether a linear quantises x in the product's own kernel: 16 rows, and room in LDS for what a workgroup keeps of them.
+// Whether a linear quantises x in the product's own kernel, which every workgroup does for its run of k, instead of a launch in
+// front of it (two microseconds or three): where that is a little.  mx_skinny_kernel with 40 KiB of LDS for it (4 rows by 9728 x
+// 2560) 9.5 us and 11.7 with the launch; mx_stream_kernel with 6 KiB (6 rows by 4096 x 12288) 10.8 and 11.4, with 10 (2 rows by 5120 x
+// 25600) 18.2 and 18.1, with 17 (8 rows by 2560 x 9728) 11.3 and 10.2, with 42 (8 rows by 5120 x 25600) 25.9 and 18.4.
 bool raw_of(int64_t rows, int64_t n, int64_t k, int format) {
     if (rows > 16) return false;
     const Form form = form_of(rows, n, k);
-    return form == kStream ? stream_raw_bytes(rows, n, k, format) <= 48 * 1024
+    return form == kStream ? stream_raw_bytes(rows, n, k, format) <= 10 * 1024
                            : form == kSkinny && skinny_raw_bytes(rows, k, format) <= 48 * 1024;
 }
 int product(const Product& p, hipStream_t stream) {

@@ -39,15 +39,24 @@ __device__ __forceinline__ f32x16 mfma32(u32x4 w, u32x4 x, f32x16 c, uint32_t w_
     return __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(a, b, c, 4, 4, BYTE, (int)w_scale, BYTE, (int)x_scale);
 }
 
+// V values of a bias from n on, those past the end any; asked for before a kernel's work, not behind it, where a request is a
+// microsecond that nothing hides.
+template <typename T, int V>
+__device__ __forceinline__ void load_bias(float (&b)[V], const typename T::elem* bias, int64_t n, int64_t N) {
+    typename T::elem e[V];
+    if (n + V <= N) {
+        __builtin_memcpy(e, bias + n, sizeof e);     // any address of the type
+    } else {
+#pragma unroll
+        for (int i = 0; i < V; ++i) e[i] = bias[n + i < N ? n + i : N - 1];
+    }
+#pragma unroll
+    for (int i = 0; i < V; ++i) b[i] = T::to_f32(e[i]);
+}
 // 4 Q consecutive values of a row of y, columns n and on, of which those below N exist.
 template <typename T, int Q>
-__device__ __forceinline__ void store_sums(f32x4 (&v)[Q], typename T::elem* y, const typename T::elem* bias, int64_t row, int64_t n,
-                                           int64_t N) {
+__device__ __forceinline__ void store_sums(const f32x4 (&v)[Q], typename T::elem* y, int64_t row, int64_t n, int64_t N) {
     typename T::elem* to = y + row * N + n;
-    if (bias) {
-#pragma unroll
-        for (int r = 0; r < 4 * Q; ++r) v[r / 4][r % 4] += T::to_f32(bias[n + r < N ? n + r : N - 1]);
-    }
     if (n + 4 * Q <= N) {
         // any address of the type
         if constexpr (sizeof(typename T::elem) == 4) {
@@ -64,13 +73,6 @@ __device__ __forceinline__ void store_sums(f32x4 (&v)[Q], typename T::elem* y, c
     for (int r = 0; r < 4 * Q - 1; ++r)
         if (n + r < N) to[r] = T::from_f32(v[r / 4][r % 4]);
 }
-template <typename T>
-__device__ __forceinline__ void store_sums(f32x4 v, typename T::elem* y, const typename T::elem* bias, int64_t row, int64_t n,
-                                           int64_t N) {
-    f32x4 one[1] = {v};
-    store_sums<T, 1>(one, y, bias, row, n, N);
-}
-
 int skinny_product(const Product& p, hipStream_t stream);       // at most 16 rows of raw x
 int64_t skinny_raw_bytes(int64_t rows, int64_t k, int format);
 int tiles_product(const Product& p, int tile, hipStream_t stream);

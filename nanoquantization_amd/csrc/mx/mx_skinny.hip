@@ -50,6 +50,8 @@ __global__ __launch_bounds__(kThreads) void mx_skinny_kernel(const void* __restr
         }
     };
     ask(wave);
+    float b[4] = {};
+    if (bias && wave < MT) load_bias<T>(b, bias, n0 + 4 * hi, N);
     if constexpr (RAW) {
         using E = typename T::elem;
         const int per_row = steps * 16;              // eights
@@ -94,12 +96,14 @@ __global__ __launch_bounds__(kThreads) void mx_skinny_kernel(const void* __restr
 #pragma unroll
     for (int j = 0; j < MT; ++j) s_acc[wave][j][lane] = acc[j];
     __syncthreads();
-    for (int j = wave; j < MT; j += kWaves) {
-        f32x4 sum = s_acc[0][j][lane];
+    if (wave < MT) {
+        f32x4 sum[1] = {s_acc[0][wave][lane]};
 #pragma unroll
-        for (int v = 1; v < kWaves; ++v) sum += s_acc[v][j][lane];
-        const int64_t row = m0 + 16 * j + lo, at = n0 + 4 * hi;
-        if (row < rows && at < N) store_sums<T>(sum, y, bias, row, at, N);
+        for (int v = 1; v < kWaves; ++v) sum[0] += s_acc[v][wave][lane];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) sum[0][i] += b[i];
+        const int64_t row = m0 + 16 * wave + lo, at = n0 + 4 * hi;
+        if (row < rows && at < N) store_sums<T>(sum, y, row, at, N);
     }
 }
 

@@ -195,6 +195,14 @@ __global__ __launch_bounds__(256 * fours(MT)) void mx_stream_kernel(const void* 
 #pragma unroll
         for (int j = 0; j < kXT; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
 
+    // Columns and bias of a lane at the end: with two fours those of its 16 bytes of a row, else four for each of its fragments.
+    constexpr int V = G::kFours == 2 ? 16 / sizeof(typename T::elem) : 4, kOf = kRows / V;
+    const int column = G::kFours == 2 ? threadIdx.x % kOf * V : wave * (16 * kWT) + 4 * hi;
+    float b[G::kFours == 2 ? 1 : kWT][V] = {};
+    if (bias && gridDim.y == 1) {
+#pragma unroll
+        for (int i = 0; i < (G::kFours == 2 ? 1 : kWT); ++i) load_bias<T>(b[i], bias, n0 + column + 16 * i, N);
+    }
     ask_scales(g0);
     load(Const<1>(), c0, 0);
     load(Const<0>(), c0 + 1, 1);
@@ -303,8 +311,8 @@ __global__ __launch_bounds__(256 * fours(MT)) void mx_stream_kernel(const void* 
     const int64_t pitch = ((int64_t)N + kRows - 1) / kRows * kRows;          // of a row of sums
     if constexpr (G::kFours == 2) {
         // The two fours' sums meet in LDS, and leave it row by row, 16 bytes a lane.  (Straight from the registers of one four a
-        // store has 32 bytes of each of 16 rows: 333 rows by 2816 x 9727 took 20.7 us, and 18.1 so.)
-        using E = typename T::elem;
+        // store has 32 bytes of each of 16 rows: 333 rows by 2816 x 9727 took 20.7 us, and 18.1 so; with a bias, asked
+        // for at the start, 20.0.)
         float* s_sum = reinterpret_cast<float*>(s_mem);
         const auto at = [&](int i, int j) {
             return reinterpret_cast<f32x4*>(s_sum + (x_row + 16 * j) * G::kSumPitch + wm * (16 * kWT) + 16 * i + 4 * hi);
@@ -324,34 +332,39 @@ __global__ __launch_bounds__(256 * fours(MT)) void mx_stream_kernel(const void* 
                 for (int i = 0; i < kWT; ++i) *at(i, j) += acc[i][j];
         }
         __syncthreads();
-        const auto rows_out = [&](auto v_, auto put) {
-            constexpr int V = decltype(v_)::value, kOf = kRows / V;          // values of a lane, lanes of a row
-            for (int e = threadIdx.x; e < rows * kOf; e += kThreads) {
-                const int r = e / kOf, c = e % kOf * V;
+        if (gridDim.y > 1) {
+            for (int e = threadIdx.x; e < rows * (kRows / 4); e += kThreads) {
+                const int r = e / (kRows / 4), c = e % (kRows / 4) * 4;
+                *reinterpret_cast<f32x4*>(sums + ((int64_t)split * all_rows + m0 + r) * pitch + n0 + c) =
+                    *reinterpret_cast<const f32x4*>(s_sum + r * G::kSumPitch + c);
+            }
+        } else if (n0 + column < N) {
+            for (int r = threadIdx.x / kOf; r < rows; r += kThreads / kOf) {
                 f32x4 v[V / 4];
 #pragma unroll
-                for (int q = 0; q < V / 4; ++q) v[q] = *reinterpret_cast<const f32x4*>(s_sum + r * G::kSumPitch + c + 4 * q);
-                if (n0 + c < N) put(v, m0 + r, n0 + c);
-            }
-        };
-        if (gridDim.y > 1) {
-            rows_out(Const<4>(), [&](f32x4 (&v)[1], int m, int n) {
-                *reinterpret_cast<f32x4*>(sums + ((int64_t)split * all_rows + m) * pitch + n) = v[0];
-            });
-        } else {
-            rows_out(Const<16 / sizeof(E)>(), [&](auto& v, int m, int n) { store_sums<T>(v, y, bias, m, n, N); });
-        }
-        return;
-    }
+                for (int q = 0; q < V / 4; ++q) {
+                    v[q] = *reinterpret_cast<const f32x4*>(s_sum + r * G::kSumPitch + column + 4 * q);
 #pragma unroll
-    for (int j = 0; j < kXT; ++j)
+                    for (int i = 0; i < 4; ++i) v[q][i] += b[0][4 * q + i];
+                }
+                store_sums<T>(v, y, m0 + r, n0 + column, N);
+            }
+        }
+    } else {
 #pragma unroll
         for (int i = 0; i < kWT; ++i) {
-            const int m = x_row + 16 * j, n = n0 + wm * (16 * kWT) + 16 * i + 4 * hi;
-            if (m >= rows || n >= N) continue;
-            if (gridDim.y > 1) *reinterpret_cast<f32x4*>(sums + ((int64_t)split * all_rows + m0 + m) * pitch + n) = acc[i][j];
-            else store_sums<T>(acc[i][j], y, bias, m0 + m, n, N);
+            const int n = n0 + column + 16 * i;
+            if (lo >= rows || n >= N) continue;
+            f32x4 v[1] = {acc[i][0]};
+            if (gridDim.y > 1) {
+                *reinterpret_cast<f32x4*>(sums + ((int64_t)split * all_rows + lo) * pitch + n) = v[0];
+            } else {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) v[0][e] += b[i][e];
+                store_sums<T>(v, y, lo, n, N);
+            }
         }
+    }
 }
 
 // y = the splits' sums, added in order, + bias.
@@ -361,19 +374,24 @@ __global__ __launch_bounds__(256) void mx_add_splits_kernel(const float* __restr
     // fewer than 160 tiles of 128 x 128 sums: 32 bits
     const uint32_t at = (blockIdx.x * 256 + threadIdx.x) * 4, m = at / (uint32_t)pitch, n = at - m * pitch;
     if (m >= (uint32_t)rows || n >= (uint32_t)N) return;
+    float b[4] = {};
+    if (bias) load_bias<T>(b, bias, n, N);
     f32x4 v = *reinterpret_cast<const f32x4*>(sums + at);
-    for (int s = 1; s < splits; s += 4) {            // four on their way at once
-        f32x4 next[4];
+    for (int s = 1; s < splits; s += 8) {            // eight on their way at once
+        f32x4 next[8];
 #pragma unroll
-        for (int u = 0; u < 4; ++u) {
+        for (int u = 0; u < 8; ++u) {
             next[u] = f32x4{0.f, 0.f, 0.f, 0.f};
             if (s + u < splits) next[u] = *reinterpret_cast<const f32x4*>(sums + (int64_t)(s + u) * rows * pitch + at);
         }
 #pragma unroll
-        for (int u = 0; u < 4; ++u)
+        for (int u = 0; u < 8; ++u)
             if (s + u < splits) v += next[u];
     }
-    store_sums<T>(v, y, bias, m, n, N);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] += b[i];
+    const f32x4 one[1] = {v};
+    store_sums<T>(one, y, m, n, N);
 }
 
 template <typename T, int FORMAT, int MT, bool RAW>
