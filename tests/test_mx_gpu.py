@@ -496,7 +496,7 @@ def _form(rows, n, k, fmt, quantised=1):
 
 # tiles of 128 and of 256: k of less than a chunk of 256, of whole ones, of both, of four and more; rows of scales of whole words or not
 TILES = [(2100, 32, 2100), (2177, 96, 2049), (2049, 256, 2100), (2100, 288, 2177), (2180, 544, 2061), (2051, 1024, 2176), (2100, 1120, 2055),
-         (2050, 2528, 2100), (2900, 32, 4096), (2817, 224, 4095), (3300, 512, 3890), (3330, 768, 3841), (2900, 1184, 4097), (2818, 2080, 4100)]
+         (2050, 2528, 2100), (2070, 384, 2090), (2060, 1152, 2100), (2900, 1408, 4096), (2900, 2176, 4090), (2900, 32, 4096), (2817, 224, 4095), (3300, 512, 3890), (3330, 768, 3841), (2900, 1184, 4097), (2818, 2080, 4100)]
 
 
 @pytest.mark.parametrize("fmt", FORMATS)
@@ -623,3 +623,18 @@ def test_more_eights_than_31_bits():
     assert bool((scales == one[1]).all())
     del x, codes, scales
     torch.cuda.empty_cache()
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("k", [128, 384, 640, 1152, 2176, 5248])
+@pytest.mark.parametrize("rows,n", [(1, 200), (16, 8200), (30, 300), (60, 140), (150, 900)])
+def test_half_a_chunk_over(rows, n, k, fmt):
+    """Rows of scales of whole words whose last four blocks are half a chunk."""
+    w, ws = _weight(n, n, k)
+    x = _random(rows, rows, k, dtype=torch.float16)
+    codes, scales = nq.mx_quantize(x, fmt)
+    y = nq.mx_linear(x, w, ws, activations=fmt)
+    _check_product(y, (codes, scales), (w, ws), None, torch.float16)
+    assert torch.equal(nq.mx_linear_quantized(codes, scales, w, ws, None, torch.float16), y)
+    off = torch.empty(scales.numel() + 1, dtype=torch.uint8, device="cuda")[1:].view_as(scales).copy_(scales)
+    assert torch.equal(nq.mx_linear_quantized(codes, off, w, ws, None, torch.float16), y)
