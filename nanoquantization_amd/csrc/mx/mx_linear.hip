@@ -22,12 +22,15 @@ int check_operands(const char* fn, const uint8_t* weight, const uint8_t* weight_
 enum Form { kSkinny, kStream, kTiles128, kTiles256 };
 
 // Which kernel runs a product.
-Form form_of(int64_t rows, int64_t n, int64_t k) {
+Form form_of(int64_t rows, int64_t n, int64_t k, int format) {
     if (k > ((int64_t)1 << 22)) return kSkinny;              // byte offsets in a tile are 32 bits
-    // One launch without a split while that is shorter than a split product and the launch that adds its sums: one row by 4096 x
-    // 12288 7.7 us and 7.1 + 1.7, by 5120 x 25600 18.7 and 12.9 + 1.3; 16 rows, which every 16 weight rows read again, by 2560 x 9728
-    // 14.7 and 8 + 2.
-    if (rows <= 4 ? n * k <= ((int64_t)64 << 20) : rows <= 16 && rows * n * k <= ((int64_t)128 << 20)) return kSkinny;
+    // One launch without a split while that is shorter than a split product and the launch that adds its sums.  One row by 4096 x
+    // 12288 8.5 us and 9.2, by 5120 x 25600 18.7 and 14.2.  More rows, which every 16 weight rows read again: e4m3 16 by 4096 x 4096
+    // 6.7 and 8.2, 16 by 2560 x 9728 8.8 and 8.9, 8 by 4096 x 12288 12.4 and 9.6, 16 by 6144 x 2048, of fewer workgroups than CUs, 8.7
+    // and 7.7; e2m1 16 by 2560 x 9728 7.3 and 9.0, 8 by 4096 x 12288 10.9 and 9.5.
+    const int64_t weight = n * k;
+    const int64_t most = format == NQX_FP4 ? (int64_t)512 << 20 : n >= 4096 ? (int64_t)256 << 20 : (int64_t)128 << 20;
+    if (rows <= 4 ? weight <= ((int64_t)64 << 20) : rows <= 16 && weight <= ((int64_t)32 << 20) && rows * weight <= most) return kSkinny;
     if (rows <= 128 || cdiv(rows, 128) * cdiv(n, 128) <= 256) return kStream;
     return cdiv(rows, 256) * cdiv(n, 256) >= 192 ? kTiles256 : kTiles128;
 }
@@ -37,12 +40,12 @@ Form form_of(int64_t rows, int64_t n, int64_t k) {
 // 25600) 18.2 and 18.1, with 17 (8 rows by 2560 x 9728) 11.3 and 10.2, with 42 (8 rows by 5120 x 25600) 25.9 and 18.4.
 bool raw_of(int64_t rows, int64_t n, int64_t k, int format) {
     if (rows > 16) return false;
-    const Form form = form_of(rows, n, k);
+    const Form form = form_of(rows, n, k, format);
     return form == kStream ? stream_raw_bytes(rows, n, k, format) <= 10 * 1024
                            : form == kSkinny && skinny_raw_bytes(rows, k, format) <= 48 * 1024;
 }
 int product(const Product& p, hipStream_t stream) {
-    switch (form_of(p.rows, p.n, p.k)) {
+    switch (form_of(p.rows, p.n, p.k, p.format)) {
         case kTiles256: return tiles_product(p, 256, stream);
         case kTiles128: return tiles_product(p, 128, stream);
         case kStream: return stream_product(p, stream);
@@ -58,7 +61,7 @@ struct Space {
 Space space_of(int64_t rows, int64_t n, int64_t k, int format, bool quantised) {
     Space s = {0, 0, 0};
     if (rows == 0 || n == 0) return s;
-    if (form_of(rows, n, k) == kStream) s.sums = stream_sums_bytes(rows, n, k);
+    if (form_of(rows, n, k, format) == kStream) s.sums = stream_sums_bytes(rows, n, k);
     if (!quantised && !raw_of(rows, n, k, format)) s.codes = (size_t)(rows * code_bytes(k, format)), s.scales = (size_t)(rows * (k / kBlock));
     return s;
 }
@@ -114,7 +117,7 @@ extern "C" int nqx_linear(const void* x, int64_t x_stride, const uint8_t* weight
 
 extern "C" const char* nqx_linear_form(int64_t rows, int64_t n, int64_t k, int dtype, int format, int quantised) {
     if (check_product("nqx_linear_form", rows, n, k, dtype, format) || rows == 0 || n == 0) return "";
-    switch (form_of(rows, n, k)) {
+    switch (form_of(rows, n, k, format)) {
         case kTiles256: return "mx_tiles_kernel 256 x 256";
         case kTiles128: return "mx_tiles_kernel 128 x 128";
         case kStream: return !quantised && raw_of(rows, n, k, format) ? "mx_stream_kernel on x as it is" : "mx_stream_kernel";

@@ -1,8 +1,11 @@
-// The product for a few rows of x, or few tiles of 128, where what counts is to stream the packed weight once: 0.53 bytes a value, and all of x
-// per workgroup.  A workgroup has 128 weight rows, all rows of x and a run of k; a wave takes a quarter of the weight rows.  Operands come to LDS by load-to-LDS in chunks of 256 values of k, whole 128-byte lines of a weight row,
-// two chunks ahead of the one that is multiplied; one barrier a chunk.  (x comes from a cache, but its requests return behind the
-// weight's: asked for one chunk ahead a chunk of 64 rows took 2.5 us.)  Where the weight has too few rows for the chip, k is split over workgroups, whose
-// sums go to memory in fp32 and are added, in the order of the splits, by a second kernel.
+// The product for a few rows of x, or few tiles of 128, where what counts is to stream the packed weight once: 0.53 bytes a value,
+// and all of x per workgroup.  A workgroup has 128 weight rows, up to 128 rows of x and a run of k.  Operands come to LDS by
+// load-to-LDS in chunks of 256 values of k, whole 128-byte lines of a weight row, two chunks ahead of the one that is multiplied;
+// one barrier a chunk.  (x comes from a cache, but its requests return behind the weight's: asked for one chunk ahead a chunk of 64
+// rows took 2.5 us.  Three chunks ahead gain nothing: 41 rows by 25600 x 5120 in 4 bits 21.6 us and 21.4.)  Where the weight has too
+// few rows for the chip, k is split over workgroups, whose sums go to memory in fp32 and are added, in the order of the splits, by a
+// second kernel.  Up to 64 rows are bound by the weight's bytes (16 by 5120 x 25600 12.3 us, 5.7 TB/s), more by what a CU gets from
+// L2 and LDS (333 by 2816 x 9728 in 8 bits 1.1 us a chunk, of which the matrix instructions need half).
 //
 // With RAW x comes as it is and every workgroup quantises its run of it into LDS first, while its first chunks are on their way:
 // one launch for a linear of few rows.
@@ -40,19 +43,21 @@ int splits_of(int64_t rows, int64_t n, int64_t k) {
 }
 template <int FORMAT, int MT, bool RAW>
 struct Stream {
-    static constexpr int kFours = fours(MT), kWaves = 4 * kFours, kThreads = 64 * kWaves, kBufs = 3, kGroup = group_chunks(MT), kBytes = 8 * kGroup;     // kBytes: a row's scales of a group
+    static constexpr int kFours = fours(MT), kWaves = 4 * kFours, kThreads = 64 * kWaves, kBufs = 3;
+    static constexpr int kGroup = group_chunks(MT), kBytes = 8 * kGroup;       // chunks whose scales come at a time, a row's bytes of them
     // fragments of a wave: four waves along the weight rows, or two along them and two along 128 rows of x
     static constexpr int kAlong = MT == 8 ? 2 : 1, kWT = kRows / 64 * kAlong, kXT = MT / kAlong;
     static constexpr int kHalves = FORMAT == NQX_FP4 ? 1 : 2;          // 128-byte parts of a row of x in a chunk
     static constexpr int kW = kRows * 128, kXHalf = 16 * MT * 128, kX = RAW ? 0 : kHalves * kXHalf, kXAt = kBufs * kW;      // [weight | x]
-    static constexpr int kWLoads = kRows / 8 / kWaves, kXAll = RAW ? 0 : 2 * MT * kHalves, kXLoads = (kXAll + kWaves - 1) / kWaves;    // of a wave, 1 KiB each
+    // load-to-LDS of a wave for a chunk, 1 KiB each
+    static constexpr int kWLoads = kRows / 8 / kWaves, kXAll = RAW ? 0 : 2 * MT * kHalves, kXLoads = (kXAll + kWaves - 1) / kWaves;
     static constexpr int kLoads = kWLoads + kXLoads;
     static constexpr int kNone = kXAt + kBufs * kX;                         // where a wave without a piece of x lets its request go
     static constexpr int kScales = kNone + (kXAll % kWaves ? 1024 : 0), kSlot = (kRows + (RAW ? 0 : 16 * MT)) * kBytes;
     static constexpr int kFixed = kScales + 2 * kSlot;
     static constexpr int kSumPitch = kRows + 4;      // floats of a row of sums of two fours, in the buffers' place
     static_assert(kFours == 1 || 16 * MT * kSumPitch * 4 <= kNone, "");
-    static_assert(kFixed * per_cu(MT) <= 160 * 1024 , "");
+    static_assert(kFixed * per_cu(MT) <= 160 * 1024, "");
 };
 // RAW: bytes of `rows` quantised rows of `chunks` chunks in LDS, codes and scales.
 __host__ __device__ constexpr int resident_bytes(int format, int rows, int chunks) {
