@@ -21,23 +21,17 @@ constexpr int kRows = 128;      // weight rows of a workgroup
 constexpr int group_chunks(int mt) { return mt >= 4 ? 2 : 4; }
 constexpr int per_cu(int mt) { return mt == 1 ? 2 : 1; }
 constexpr int fours(int mt) { return mt == 1 ? 1 : 2; }
-// The most chunks that one of `splits` runs has.
-int most_chunks(int chunks, int blocks, int splits, int group) {
-    const int first = blocks & 7 ? 1 : 0, whole = chunks - first, groups = first + (whole + group - 1) / group;
-    const int most = group * (int)cdiv(groups, splits);
-    return most < chunks ? most : chunks;
-}
+int chunks_of(int64_t k) { return (int)cdiv(k, 256); }
 int sixteens(int64_t rows) { return rows <= 16 ? 1 : rows <= 32 ? 2 : rows <= 64 ? 4 : 8; }
 // Splits of k: none where 160 workgroups do without (the sums of splits cost another launch), else as many as fill the chip with
-// workgroups that are resident at once, of a group of chunks and four chunks each at least.  (Workgroups of 256 weight rows would
-// share x among more of them: 41 rows by 25600 x 5120 26.5 us and 24.5 with 128, 64 rows by 4096 x 12288 17.6 and 14.3; eight
-// splits of two chunks instead of four of four, 64 rows by 4096 x 4096, 12.2 and 10.7.)
+// workgroups that are resident at once, of four chunks each at least.  (Workgroups of 256 weight rows would share x among more of
+// them: 41 rows by 25600 x 5120 26.5 us and 24.5 with 128, 64 rows by 4096 x 12288 17.6 and 14.3; eight splits of two chunks instead
+// of four of four, 64 rows by 4096 x 4096, 12.2 and 10.7.)
 int splits_of(int64_t rows, int64_t n, int64_t k) {
-    const int mt = sixteens(rows), per = group_chunks(mt);
-    const int64_t blocks = k / kBlock, groups = (blocks & 7 ? 1 : 0) + ((blocks >> 3) + per - 1) / per, tiles = cdiv(n, kRows) * cdiv(rows, 16 * mt);
+    const int mt = sixteens(rows);
+    const int64_t tiles = cdiv(n, kRows) * cdiv(rows, 16 * mt);
     int64_t s = tiles >= 160 ? 1 : 256 * per_cu(mt) / tiles;
-    if (s > groups) s = groups;
-    if (s > (blocks >> 5)) s = blocks >> 5;
+    if (s > k / 1024) s = k / 1024;
     if (s > 16) s = 16;
     return s < 1 ? 1 : (int)s;
 }
@@ -68,8 +62,8 @@ template <typename T, int FORMAT, int MT, bool RAW>
 __global__ __launch_bounds__(256 * fours(MT)) void mx_stream_kernel(const void* __restrict__ x, int64_t x_stride, const uint8_t* __restrict__ xs,
                                                         const uint8_t* __restrict__ w, const uint8_t* __restrict__ ws,
                                                         const typename T::elem* __restrict__ bias, typename T::elem* __restrict__ y,
-                                                        float* __restrict__ sums, int rows, int N, int blocks, int words, int groups_each,
-                                                        int groups_more, uint32_t row_tiles) {
+                                                        float* __restrict__ sums, int rows, int N, int blocks, int words, int each, int more,
+                                                        uint32_t row_tiles) {
     using G = Stream<FORMAT, MT, RAW>;
     constexpr bool kFour = FORMAT == NQX_FP4;
     constexpr int kWaves = G::kWaves, kThreads = G::kThreads, kWT = G::kWT, kXT = G::kXT, kGroup = G::kGroup, kBytes = G::kBytes;
@@ -85,12 +79,13 @@ __global__ __launch_bounds__(256 * fours(MT)) void mx_stream_kernel(const void* 
     rows = rows - m0 < 16 * MT ? rows - m0 : 16 * MT;
     const uint32_t w_pitch = (uint32_t)blocks * 16, x_pitch = (uint32_t)blocks * (kFour ? 16 : 32);
     // Chunks: the blocks that do not fill one come first (pieces that do not exist are asked for past the buffer's end, which
-    // leaves zeros), then the whole ones.  Scales come for a group of chunks at a time, kBytes of a row: for the chunk that is
-    // not whole, then for kGroup whole ones each.  A split has whole groups, the first groups_more of them one more than the others.
+    // leaves zeros), then the whole ones.  A split has a run of them, the first `more` splits one more than the others.  Scales come for
+    // a group of chunks at a time, kBytes of a row: for the chunk that is not whole, then for kGroup whole ones each.
     const int part = blocks & 7, whole = blocks >> 3, first = part ? 1 : 0;
-    const int g0 = split * groups_each + min(split, groups_more), g1 = g0 + groups_each + (split < groups_more ? 1 : 0);
-    const auto chunk_of = [&](int g) { return g < first ? 0 : min(first + kGroup * (g - first), first + whole); };
-    const int c0 = chunk_of(g0), c1 = chunk_of(g1);
+    const int c0 = split * each + min(split, more), c1 = c0 + each + (split < more ? 1 : 0);
+    const auto group_of = [&](int c) { return c < first ? 0 : first + (c - first) / kGroup; };
+    const auto chunk_of = [&](int g) { return g < first ? 0 : first + kGroup * (g - first); };       // a group's first
+    const int g0 = group_of(c0), g1 = group_of(c1 - 1) + 1;
 
     const uint8_t *wb = w + (int64_t)n0 * w_pitch, *wsb = ws + (int64_t)n0 * blocks, *xb = static_cast<const uint8_t*>(x) + (RAW ? 0 : (int64_t)m0 * x_pitch);
     if constexpr (!RAW) xs += (int64_t)m0 * blocks;
@@ -404,18 +399,17 @@ hipError_t launch(const Product& p, hipStream_t stream) {
     using G = Stream<FORMAT, MT, RAW>;
     using E = typename T::elem;
     const int blocks = (int)(p.k / kBlock), tiles = (int)cdiv(p.n, kRows), splits = splits_of(p.rows, p.n, p.k);
-    const int chunks = (blocks & 7 ? 1 : 0) + (blocks >> 3);
-    const int lds = G::kFixed + (RAW ? resident_bytes(FORMAT, (int)p.rows, most_chunks(chunks, blocks, splits, G::kGroup)) : 0);
+    const int chunks = chunks_of(p.k);
+    const int lds = G::kFixed + (RAW ? resident_bytes(FORMAT, (int)p.rows, (int)cdiv(chunks, splits)) : 0);
     if (lds > 64 * 1024)
         if (const hipError_t e = allow_lds<&mx_stream_kernel<T, FORMAT, MT, RAW>>(160 * 1024); e != hipSuccess) return e;
     const int words = blocks % 4 == 0 && blocks >= G::kBytes && ((reinterpret_cast<uintptr_t>(p.ws) | reinterpret_cast<uintptr_t>(p.xs)) & 3) == 0;
     const E *bias = static_cast<const E*>(p.bias);
     E* y = static_cast<E*>(p.y);
-    const int groups = (blocks & 7 ? 1 : 0) + ((blocks >> 3) + G::kGroup - 1) / G::kGroup;
     const unsigned row_tiles = (unsigned)cdiv(p.rows, 16 * MT);
     const dim3 grid(row_tiles == 1 ? tiles : cdiv(tiles, 8) * 8 * row_tiles, splits);
     const hipError_t e = start(&mx_stream_kernel<T, FORMAT, MT, RAW>, grid, G::kThreads, lds, stream, RAW ? p.raw : p.x, p.raw_stride, p.xs,
-                               p.w, p.ws, bias, y, p.sums, (int)p.rows, (int)p.n, blocks, words, groups / splits, groups % splits, row_tiles);
+                               p.w, p.ws, bias, y, p.sums, (int)p.rows, (int)p.n, blocks, words, chunks / splits, chunks % splits, row_tiles);
     if (e != hipSuccess || splits == 1) return e;
     const int pitch = tiles * kRows;
     return start(&mx_add_splits_kernel<T>, dim3((unsigned)cdiv(p.rows * pitch, 1024)), 256, 0, stream, p.sums, bias, y, (int)p.rows, (int)p.n,
@@ -444,8 +438,7 @@ size_t stream_sums_bytes(int64_t rows, int64_t n, int64_t k) {
     return splits > 1 ? (size_t)(splits * rows * cdiv(n, kRows) * kRows * 4) : 0;
 }
 int stream_raw_bytes(int64_t rows, int64_t n, int64_t k, int format) {
-    const int blocks = (int)(k / kBlock), chunks = (blocks & 7 ? 1 : 0) + (blocks >> 3);
-    return resident_bytes(format, (int)rows, most_chunks(chunks, blocks, splits_of(rows, n, k), group_chunks(1)));
+    return resident_bytes(format, (int)rows, (int)cdiv(chunks_of(k), splits_of(rows, n, k)));
 }
 
 }  // namespace nqx
