@@ -24,13 +24,16 @@ enum Form { kSkinny, kStream, kTiles128, kTiles256 };
 // Which kernel runs a product.
 Form form_of(int64_t rows, int64_t n, int64_t k, int format) {
     if (k > ((int64_t)1 << 22)) return kSkinny;              // byte offsets in a tile are 32 bits
-    // One launch without a split while that is shorter than a split product and the launch that adds its sums.  One row by 4096 x
-    // 12288 8.5 us and 9.2, by 5120 x 25600 18.7 and 14.2.  More rows, which every 16 weight rows read again: e4m3 16 by 4096 x 4096
-    // 6.7 and 8.2, 16 by 2560 x 9728 8.8 and 8.9, 8 by 4096 x 12288 12.4 and 9.6, 16 by 6144 x 2048, of fewer workgroups than CUs, 8.7
-    // and 7.7; e2m1 16 by 2560 x 9728 7.3 and 9.0, 8 by 4096 x 12288 10.9 and 9.5.
-    const int64_t weight = n * k;
-    const int64_t most = format == NQX_FP4 ? (int64_t)512 << 20 : n >= 4096 ? (int64_t)256 << 20 : (int64_t)128 << 20;
-    if (rows <= 4 ? weight <= ((int64_t)64 << 20) : rows <= 16 && weight <= ((int64_t)32 << 20) && rows * weight <= most) return kSkinny;
+    // One launch without a split while that is shorter than a split product and the launch that adds its sums.  One row by 4096 x 4096
+    // 4.8 us and 8.0, by 4096 x 12288 8.5 and 9.2, by 5120 x 12288 10.0 and 9.8.  Long rows are many rounds of a few workgroups: by
+    // 9728 x 1024 6.6 and 7.2, by 12288 x 1024 9.0 and 7.3, by 25600 x 256 15.4 and 8.2; and where they are a multiple of 4 KiB apart,
+    // 16 of them at a time ask the same channels: by 8192 x 5120 11.0 and 9.0.  More rows, which every 16 weight rows read again:
+    // e4m3 16 by 4096 x 4096 6.7 and 8.2, 8 by 2560 x 9728 7.3 and 8.9, 8 by 4096 x 8192 9.1 and 7.6, 8 by 9728 x 1024 8.6 and 7.1; e2m1
+    // 16 by 2560 x 9728 7.3 and 9.0.
+    const int64_t weight = n * k, Mi = (int64_t)1 << 20;
+    const bool one = rows <= 4 ? k <= 10240 && weight <= 48 * Mi
+                               : rows <= 16 && k <= 6144 && weight <= 24 * Mi && rows * weight <= (format == NQX_FP4 ? 512 : n >= 4096 ? 256 : 128) * Mi;
+    if (one && k % 8192 != 0) return kSkinny;
     // One round of workgroups with eight waves each, while there is one: 256 tiles of 128 (1024 rows by 4096 x 4096) in 8 bits 23.3 us
     // and 28.4 by tiles, in 4 bits 18.6 and 17.4; of 288 (1100 rows) 42.0 and 35.9, 34.1 and 21.5.
     if (rows <= 128 || cdiv(rows, 128) * cdiv(n, 128) <= 256) return kStream;
