@@ -35,8 +35,11 @@ Form form_of(int64_t rows, int64_t n, int64_t k, int format) {
                                : rows <= 16 && k <= 6144 && weight <= 24 * Mi && rows * weight <= (format == NQX_FP4 ? 512 : n >= 4096 ? 256 : 128) * Mi;
     if (one && k % 8192 != 0) return kSkinny;
     // One round of workgroups with eight waves each, while there is one: 256 tiles of 128 (1024 rows by 4096 x 4096) in 8 bits 23.3 us
-    // and 28.4 by tiles, in 4 bits 18.6 and 17.4; of 288 (1100 rows) 42.0 and 35.9, 34.1 and 21.5.
-    if (rows <= 128 || cdiv(rows, 128) * cdiv(n, 128) <= 256) return kStream;
+    // and 28.4 by tiles; of 288 (1100 rows) 42.0 and 35.9.  Where k is not split tiles are better off in 4 bits, whose fragments they
+    // read a step ahead, but for weights that take longer to come: 200 rows by 1024 x 4096 8.1 and 6.1, 1000 by 4096 x 4096 18.5 and
+    // 16.0, 128 by 4096 x 12288 16.9 and 15.5, by 5120 x 12288 21.9 and 25.9.
+    const bool round = rows <= 128 || cdiv(rows, 128) * cdiv(n, 128) <= 256;
+    if (round && (format == NQX_FP8 || rows <= 64 || weight > 48 * Mi || stream_splits(rows, n, k, format))) return kStream;
     // Tiles of 256 need half the bytes a product; too few of them leave CUs idle: 128 (2000 by 4096 x 4096) in 8 bits 57.8 us and 39.9 of
     // 128, 176 (2800 rows) 57.7 and 53.9, 200 (333 by 4096 x 25600) 61.2 and 62.6, 224 (3584 rows) 59.0 and 65.6.
     return cdiv(rows, 256) * cdiv(n, 256) >= 192 ? kTiles256 : kTiles128;
@@ -68,7 +71,7 @@ struct Space {
 Space space_of(int64_t rows, int64_t n, int64_t k, int format, bool quantised) {
     Space s = {0, 0, 0};
     if (rows == 0 || n == 0) return s;
-    if (form_of(rows, n, k, format) == kStream) s.sums = stream_sums_bytes(rows, n, k);
+    if (form_of(rows, n, k, format) == kStream) s.sums = stream_sums_bytes(rows, n, k, format);
     if (!quantised && !raw_of(rows, n, k, format)) s.codes = (size_t)(rows * code_bytes(k, format)), s.scales = (size_t)(rows * (k / kBlock));
     return s;
 }

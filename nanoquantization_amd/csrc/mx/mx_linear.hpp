@@ -77,7 +77,8 @@ int skinny_product(const Product& p, hipStream_t stream);       // at most 16 ro
 int64_t skinny_raw_bytes(int64_t rows, int64_t k, int format);
 int tiles_product(const Product& p, int tile, hipStream_t stream);
 int stream_product(const Product& p, hipStream_t stream);       // at most 128 rows, at most 16 of raw x
-size_t stream_sums_bytes(int64_t rows, int64_t n, int64_t k);
+bool stream_splits(int64_t rows, int64_t n, int64_t k, int format);
+size_t stream_sums_bytes(int64_t rows, int64_t n, int64_t k, int format);
 int stream_raw_bytes(int64_t rows, int64_t n, int64_t k, int format);
 
 }  // namespace nqx

@@ -23,17 +23,23 @@ constexpr int per_cu(int mt) { return mt == 1 ? 2 : 1; }
 constexpr int fours(int mt) { return mt == 1 ? 1 : 2; }
 int chunks_of(int64_t k) { return (int)cdiv(k, 256); }
 int sixteens(int64_t rows) { return rows <= 16 ? 1 : rows <= 32 ? 2 : rows <= 64 ? 4 : 8; }
-// Splits of k: none where 160 workgroups do without (the sums of splits cost another launch), else as many as fill the chip with
-// workgroups that are resident at once, of four chunks each at least.  (Workgroups of 256 weight rows would share x among more of
-// them: 41 rows by 25600 x 5120 26.5 us and 24.5 with 128, 64 rows by 4096 x 12288 17.6 and 14.3; eight splits of two chunks instead
-// of four of four, 64 rows by 4096 x 4096, 12.2 and 10.7.)
-int splits_of(int64_t rows, int64_t n, int64_t k) {
+// Splits of k: at most as many as fill the chip with workgroups that are resident at once, of four chunks each at least, and of those
+// the number that costs least: the longest split's chunks, and where there is more than one a launch and the sums' way to memory
+// and back.  Nanoseconds of a chunk and of a launch as measured; 128 rows by 2560 x 9728 in 8 bits 18.0 us with two splits and 15.2
+// with one, 64 rows in 4 bits 11.7 and 9.5.  (Workgroups of 256 weight rows would share x among more of them: 41 rows by
+// 25600 x 5120 26.5 us and 24.5 with 128, 64 rows by 4096 x 12288 17.6 and 14.3.)
+int splits_of(int64_t rows, int64_t n, int64_t k, int format) {
     const int mt = sixteens(rows);
-    const int64_t tiles = cdiv(n, kRows) * cdiv(rows, 16 * mt);
-    int64_t s = tiles >= 160 ? 1 : 256 * per_cu(mt) / tiles;
-    if (s > k / 1024) s = k / 1024;
-    if (s > 16) s = 16;
-    return s < 1 ? 1 : (int)s;
+    const int64_t tiles = cdiv(n, kRows) * cdiv(rows, 16 * mt), chunks = chunks_of(k), chunk = mt == 8 ? (format == NQX_FP4 ? 730 : 1070) : mt == 4 ? 700 : 600;
+    int64_t most = 256 * per_cu(mt) / tiles;
+    if (most > k / 1024) most = k / 1024;
+    if (most > 16) most = 16;
+    int64_t best = 1, time = chunks * chunk;
+    for (int64_t s = 2; s <= most; ++s) {
+        const int64_t t = cdiv(chunks, s) * chunk + 3000 + s * rows * n * 8 / 5200;
+        if (t < time) best = s, time = t;
+    }
+    return (int)best;
 }
 template <int FORMAT, int MT, bool RAW>
 struct Stream {
@@ -398,7 +404,7 @@ template <typename T, int FORMAT, int MT, bool RAW>
 hipError_t launch(const Product& p, hipStream_t stream) {
     using G = Stream<FORMAT, MT, RAW>;
     using E = typename T::elem;
-    const int blocks = (int)(p.k / kBlock), tiles = (int)cdiv(p.n, kRows), splits = splits_of(p.rows, p.n, p.k);
+    const int blocks = (int)(p.k / kBlock), tiles = (int)cdiv(p.n, kRows), splits = splits_of(p.rows, p.n, p.k, FORMAT);
     const int chunks = chunks_of(p.k);
     const int lds = G::kFixed + (RAW ? resident_bytes(FORMAT, (int)p.rows, (int)cdiv(chunks, splits)) : 0);
     if (lds > 64 * 1024)
@@ -433,12 +439,13 @@ int stream_product(const Product& p, hipStream_t stream) {
     return hip_status("mx_stream_kernel", e);
 }
 
-size_t stream_sums_bytes(int64_t rows, int64_t n, int64_t k) {
-    const int64_t splits = splits_of(rows, n, k);
+bool stream_splits(int64_t rows, int64_t n, int64_t k, int format) { return splits_of(rows, n, k, format) > 1; }
+size_t stream_sums_bytes(int64_t rows, int64_t n, int64_t k, int format) {
+    const int64_t splits = splits_of(rows, n, k, format);
     return splits > 1 ? (size_t)(splits * rows * cdiv(n, kRows) * kRows * 4) : 0;
 }
 int stream_raw_bytes(int64_t rows, int64_t n, int64_t k, int format) {
-    return resident_bytes(format, (int)rows, (int)cdiv(chunks_of(k), splits_of(rows, n, k)));
+    return resident_bytes(format, (int)rows, (int)cdiv(chunks_of(k), splits_of(rows, n, k, format)));
 }
 
 }  // namespace nqx
