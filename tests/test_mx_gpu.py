@@ -638,3 +638,21 @@ def test_half_a_chunk_over(rows, n, k, fmt):
     assert torch.equal(nq.mx_linear_quantized(codes, scales, w, ws, None, torch.float16), y)
     off = torch.empty(scales.numel() + 1, dtype=torch.uint8, device="cuda")[1:].view_as(scales).copy_(scales)
     assert torch.equal(nq.mx_linear_quantized(codes, off, w, ws, None, torch.float16), y)
+
+
+@pytest.mark.parametrize("dt", ["bf16", "f32"])
+@pytest.mark.parametrize("rows,k,n,fmt,form", [
+    (4, 1056, 700, "mxfp4", "skinny"), (16, 2080, 300, "mxfp8", "skinny"), (3, 8192, 130, "mxfp8", "stream"), (2, 12320, 70, "mxfp4", "stream"),
+    (16, 544, 60001, "mxfp8", "stream"), (30, 544, 513, "mxfp4", "stream"), (60, 4128, 257, "mxfp8", "stream"), (70, 544, 100001, "mxfp4", "stream"),
+    (120, 6176, 259, "mxfp4", "stream"), (200, 4128, 12701, "mxfp4", "stream"), (300, 1056, 515, "mxfp8", "stream"), (129, 1056, 515, "mxfp4", "tiles")])
+def test_every_kernel_with_and_without_a_bias(rows, k, n, fmt, form, dt):
+    """Of x quantised before and on the way; which kernel runs is said, so that none goes untested when a rule moves."""
+    t = DT[dt]
+    assert _form(rows, n, k, fmt).startswith(f"mx_{form}_kernel")
+    w, ws = _weight(n, n, k)
+    x = _random(rows, rows, k, dtype=t)
+    codes, scales = nq.mx_quantize(x, fmt)
+    for bias in (None, _random(k, n + 1, dtype=t, spread=False)[1:]):
+        y = nq.mx_linear_quantized(codes, scales, w, ws, bias, t)
+        _check_product(y, (codes, scales), (w, ws), bias, t)
+        assert torch.equal(nq.mx_linear(x, w, ws, bias, fmt), y)
