@@ -24,20 +24,24 @@ constexpr int fours(int mt) { return mt == 1 ? 1 : 2; }
 int chunks_of(int64_t k) { return (int)cdiv(k, 256); }
 int sixteens(int64_t rows) { return rows <= 16 ? 1 : rows <= 32 ? 2 : rows <= 64 ? 4 : 8; }
 // Splits of k: at most as many as fill the chip with workgroups that are resident at once, of four chunks each at least, and of those
-// the number that costs least: the longest split's chunks, and where there is more than one a launch and the sums' way to memory
-// and back.  Nanoseconds of a chunk and of a launch as measured; 128 rows by 2560 x 9728 in 8 bits 18.0 us with two splits and 15.2
-// with one, 64 rows in 4 bits 11.7 and 9.5.  (Workgroups of 256 weight rows would share x among more of them: 41 rows by
+// the number that costs least: the longest split's chunks or, if that is more, the weight's way from memory, and where there is more
+// than one a launch and the sums' way to memory and back.  Nanoseconds of a chunk and of a launch and 5.2 TB/s as measured; 128 rows by 2560 x 9728 in 8 bits 18.0 us with two splits and 15.2
+// with one, 64 rows in 4 bits 11.7 and 9.5; 16 rows by 5120 x 25600 17.9
+// and 15.2.  (Workgroups of 256 weight rows would share x among more of them: 41 rows by
 // 25600 x 5120 26.5 us and 24.5 with 128, 64 rows by 4096 x 12288 17.6 and 14.3.)
 int splits_of(int64_t rows, int64_t n, int64_t k, int format) {
     const int mt = sixteens(rows);
-    const int64_t tiles = cdiv(n, kRows) * cdiv(rows, 16 * mt), chunks = chunks_of(k), chunk = mt == 8 ? (format == NQX_FP4 ? 730 : 1070) : mt == 4 ? 700 : 600;
+    const int64_t tiles = cdiv(n, kRows) * cdiv(rows, 16 * mt), chunks = chunks_of(k), chunk = mt == 8 ? (format == NQX_FP4 ? 730 : 1070) : mt == 1 ? 600 : 700;
     int64_t most = 256 * per_cu(mt) / tiles;
     if (most > k / 1024) most = k / 1024;
     if (most > 16) most = 16;
-    int64_t best = 1, time = chunks * chunk;
-    for (int64_t s = 2; s <= most; ++s) {
-        const int64_t t = cdiv(chunks, s) * chunk + 3000 + s * rows * n * 8 / 5200;
-        if (t < time) best = s, time = t;
+    const int64_t least = n * (k * 17 / 32) / 5200;          // the weight's way from memory
+    int64_t best = 1, time = 0;
+    for (int64_t s = 1; s <= most || s == 1; ++s) {
+        int64_t t = cdiv(chunks, s) * chunk;
+        if (t < least) t = least;
+        if (s > 1) t += 3000 + s * rows * n * 8 / 5200;
+        if (s == 1 || t < time) best = s, time = t;
     }
     return (int)best;
 }
