@@ -40,9 +40,13 @@ Form form_of(int64_t rows, int64_t n, int64_t k, int format) {
     // 16.0, 128 by 4096 x 12288 16.9 and 15.5, by 5120 x 12288 21.9 and 25.9.
     const bool round = rows <= 128 || cdiv(rows, 128) * cdiv(n, 128) <= 256;
     if (round && (format == NQX_FP8 || rows <= 64 || weight > 48 * Mi || stream_splits(rows, n, k, format))) return kStream;
-    // Tiles of 256 need half the bytes a product; too few of them leave CUs idle: 128 (2000 by 4096 x 4096) in 8 bits 57.8 us and 39.9 of
-    // 128, 176 (2800 rows) 57.7 and 53.9, 200 (333 by 4096 x 25600) 61.2 and 62.6, 224 (3584 rows) 59.0 and 65.6.
-    return cdiv(rows, 256) * cdiv(n, 256) >= 192 ? kTiles256 : kTiles128;
+    // Tiles of 256 need half the bytes a product, tiles of 128 waste less where the last round of workgroups is not full (two of them
+    // fit a CU).  In tenths of the time of 256 tiles of 128 a round of 256 tiles of 256 takes 33 (e2m1) or 35 (e4m3), one of 512 of 128
+    // 20, and a last one of up to 256 of them 13 or 11: 8192 by 4096 x 12288 in 4 bits 238 us and 288 by tiles of 128, in 8 bits 359 and
+    // 410; 3151 by 1024 x 20480 75 and 61, 104 and 87; 3000 by 4096 x 4096 34.6 and 35.9, 59.3 and 54.9.
+    const int64_t wide = cdiv(rows, 256) * cdiv(n, 256), small = cdiv(rows, 128) * cdiv(n, 128), last = small % 512;
+    const bool four = format == NQX_FP4;
+    return cdiv(wide, 256) * (four ? 33 : 35) <= small / 512 * 20 + (last == 0 ? 0 : last > 256 ? 20 : four ? 13 : 11) ? kTiles256 : kTiles128;
 }
 // Whether a linear quantises x in the product's own kernel, which every workgroup does for its run of k, instead of a launch in
 // front of it (two microseconds or three): where that is a little.  mx_skinny_kernel with 40 KiB of LDS for it (4 rows by 9728 x

@@ -80,10 +80,10 @@ __global__ __launch_bounds__(256 * fours(MT)) void mx_stream_kernel(const void* 
     extern __shared__ __attribute__((aligned(16))) unsigned char s_mem[];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lo = lane & 15, hi = lane >> 4;
     // The row tiles of a weight tile run next to each other on one XCD (workgroups go round the eight of them), whose L2 then has
-    // the weight for all but the first: 333 rows by 2816 x 9728 in 8 bits 17.8 us, 18.1 across
-    // XCDs; 1000 by 4096 x 4096 24.5 and 26.5.
+    // the weight for all but the first: 333 rows by 2816 x 9728 in 8 bits 17.8 us, 18.1 across XCDs; 1000 by 4096 x 4096 24.5 and 26.5.
+    // row_tiles is 1 where they lie along blockIdx.z: one tile, or an XCD would have more workgroups than CUs.
     const uint32_t turn = blockIdx.x >> 3, tile = row_tiles == 1 ? blockIdx.x : turn / row_tiles * 8 + (blockIdx.x & 7);
-    const int split = blockIdx.y, n0 = (int)(tile * kRows), m0 = row_tiles == 1 ? 0 : (int)(turn % row_tiles) * (16 * MT);
+    const int split = blockIdx.y, n0 = (int)(tile * kRows), m0 = (int)(row_tiles == 1 ? blockIdx.z : turn % row_tiles) * (16 * MT);
     if (n0 >= N) return;
     const int n_rows = N - n0 < kRows ? N - n0 : kRows, all_rows = rows;
     rows = rows - m0 < 16 * MT ? rows - m0 : 16 * MT;
@@ -416,8 +416,8 @@ hipError_t launch(const Product& p, hipStream_t stream) {
     const int words = blocks % 4 == 0 && blocks >= G::kBytes && ((reinterpret_cast<uintptr_t>(p.ws) | reinterpret_cast<uintptr_t>(p.xs)) & 3) == 0;
     const E *bias = static_cast<const E*>(p.bias);
     E* y = static_cast<E*>(p.y);
-    const unsigned row_tiles = (unsigned)cdiv(p.rows, 16 * MT);
-    const dim3 grid(row_tiles == 1 ? tiles : cdiv(tiles, 8) * 8 * row_tiles, splits);
+    const unsigned all = (unsigned)cdiv(p.rows, 16 * MT), row_tiles = cdiv(tiles, 8) * all * splits <= 32 ? all : 1;
+    const dim3 grid(row_tiles == 1 ? tiles : cdiv(tiles, 8) * 8 * row_tiles, splits, row_tiles == 1 ? all : 1);
     const hipError_t e = start(&mx_stream_kernel<T, FORMAT, MT, RAW>, grid, G::kThreads, lds, stream, RAW ? p.raw : p.x, p.raw_stride, p.xs,
                                p.w, p.ws, bias, y, p.sums, (int)p.rows, (int)p.n, blocks, words, chunks / splits, chunks % splits, row_tiles);
     if (e != hipSuccess || splits == 1) return e;

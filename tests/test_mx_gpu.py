@@ -496,7 +496,7 @@ def _form(rows, n, k, fmt, quantised=1):
 
 # tiles of 128 and of 256: k of less than a chunk of 256, of whole ones, of both, of four and more; rows of scales of whole words or not
 TILES = [(2100, 32, 2100), (2177, 96, 2049), (2049, 256, 2100), (2100, 288, 2177), (2180, 544, 2061), (2051, 1024, 2176), (2100, 1120, 2055),
-         (2050, 2528, 2100), (2070, 384, 2090), (2060, 1152, 2100), (2900, 1408, 4096), (2900, 2176, 4090), (2900, 32, 4096), (2817, 224, 4095), (3300, 512, 3890), (3330, 768, 3841), (2900, 1184, 4097), (2818, 2080, 4100)]
+         (2050, 2528, 2100), (2070, 384, 2090), (2060, 1152, 2100), (3500, 1408, 4096), (3500, 2176, 4090), (3500, 32, 4096), (3457, 224, 4095), (3300, 512, 3890), (3330, 768, 3841), (3500, 1184, 4097), (3460, 2080, 4100)]
 
 
 @pytest.mark.parametrize("fmt", FORMATS)
@@ -516,7 +516,7 @@ def test_tiles(rows, k, n, fmt):
 
 
 @pytest.mark.parametrize("fmt", FORMATS)
-@pytest.mark.parametrize("rows,k,n", [(2100, 1184, 2100), (2900, 1184, 4096), (2900, 1024, 4096)])
+@pytest.mark.parametrize("rows,k,n", [(2100, 1184, 2100), (3500, 1184, 4096), (3500, 1024, 4096)])
 def test_tiles_of_every_code(rows, k, n, fmt):
     g = _gen(rows + k)
     w = torch.randint(0, 256, (n, k // 2), device="cuda", generator=g, dtype=torch.uint8)
@@ -529,7 +529,7 @@ def test_tiles_of_every_code(rows, k, n, fmt):
 
 
 @pytest.mark.parametrize("fmt", FORMATS)
-@pytest.mark.parametrize("rows,k,n", [(2100, 1120, 2100), (2900, 1120, 4100)])
+@pytest.mark.parametrize("rows,k,n", [(2100, 1120, 2100), (3500, 1120, 4100)])
 def test_nan_stays_in_its_rows_of_tiles(rows, k, n, fmt):
     w, ws = _weight(5, n, k)
     codes, scales = nq.mx_quantize(_random(6, rows, k), fmt)
@@ -656,3 +656,13 @@ def test_every_kernel_with_and_without_a_bias(rows, k, n, fmt, form, dt):
         y = nq.mx_linear_quantized(codes, scales, w, ws, bias, t)
         _check_product(y, (codes, scales), (w, ws), bias, t)
         assert torch.equal(nq.mx_linear(x, w, ws, bias, fmt), y)
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("rows,k,n", [(2000, 2080, 1000), (700, 9760, 1147), (400, 9728, 2560)])
+def test_row_tiles_across_xcds(rows, k, n, fmt):
+    """More row tiles of a weight tile than an XCD has room for, with splits of k and without."""
+    w, ws = _weight(n, n, k)
+    codes, scales = nq.mx_quantize(_random(rows, rows, k), fmt)
+    bias = _random(k, n, spread=False)
+    _check_product(nq.mx_linear_quantized(codes, scales, w, ws, bias), (codes, scales), (w, ws), bias, torch.bfloat16)
