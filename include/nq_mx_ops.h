@@ -73,8 +73,9 @@ int nqx_add_rmsnorm(const void* x, int64_t x_stride, const void* delta, int64_t 
                     void* total, uint8_t* codes, uint8_t* scales, int64_t rows, int64_t k, float eps, int dtype, int format,
                     void* stream);
 
-/* codes, scales of SiLU(gate) * up = gate / (1 + exp(-gate)) * up, computed in fp32; gate and up [rows, k], rows gate_stride
- * and up_stride apart (2 k for the halves of one tensor). */
+/* codes, scales of SiLU(gate) * up = gate / (1 + exp(-gate)) * up, computed in fp32, as gate * exp(gate) * up where gate is far below
+ * zero: a result is right wherever it is one of fp32's, also of gates whose exp(-gate) is past fp32.  A gate of -inf gives NaN.
+ * gate and up [rows, k], rows gate_stride and up_stride apart (2 k for the halves of one tensor). */
 int nqx_silu_mul(const void* gate, int64_t gate_stride, const void* up, int64_t up_stride, uint8_t* codes, uint8_t* scales,
                  int64_t rows, int64_t k, int dtype, int format, void* stream);
 

@@ -154,13 +154,26 @@ __global__ __launch_bounds__(kThreads) void mx_add_rmsnorm_kernel(const typename
 // gate / (1 + exp(-gate)) * up.  exp(-g) is 2^t 2^r, t = -g log2(e) rounded and r what that and the constant lost: without r the
 // relative error grows with |g|.  (2^r as a factor of its own near 1: where 2^t is infinite a sum could be inf - inf.)  The
 // reciprocal is off by a step of fp32 at most, a division would be by half of one and takes ten times as long (8192 x 12288 bf16
-// to e2m1 is 102 us, 4.5 TB/s, and was 116 with expf and a division).  Past 100 the exponential is infinite or does not change 1.
+// to e2m1 is 102 us, 4.5 TB/s, and was 116 with expf and a division).  Above 100 the exponential does not change 1.  For gates
+// below kFar the result is silu_mul_far's: the hardware reciprocal has no subnormal results, so from -87.3 on it would be 0, which a
+// large `up` would make of values that are not small.
+constexpr float kHigh = 1.44269502f, kLow = 1.92596303e-8f;       // log2(e) in two parts
+constexpr float kFar = -80.f;
 __device__ __forceinline__ float silu_mul(float gate, float up) {
-    constexpr float kHigh = 1.44269502f, kLow = 1.92596303e-8f, kLn2 = 0.693147182f;
+    constexpr float kLn2 = 0.693147182f;
     const float g = -__builtin_amdgcn_fmed3f(gate, -100.f, 100.f), t = g * kHigh;
     const float r = __builtin_fmaf(g, kLow, __builtin_fmaf(g, kHigh, -t));
     const float e = __builtin_amdgcn_exp2f(t) * __builtin_fmaf(r, kLn2, 1.0f);
     return gate * __builtin_amdgcn_rcpf(1.0f + e) * up;
+}
+// The same for gates below kFar, where 1 + exp(-gate) is exp(-gate) in fp32: gate * exp(gate) * up, its powers of two last, so that
+// nothing under- or overflows that the result does not.  exp(gate) is 2^n 2^f, n = gate log2(e) rounded to a whole number.  (Gates below
+// -1000 are 0 times any `up`; -inf stays, a NaN as inf / inf is.)
+__device__ __forceinline__ float silu_mul_far(float gate, float up) {
+    const float g = fmaxf(gate, -1000.f), n = __builtin_rintf(g * kHigh);
+    const float f = __builtin_fmaf(g, kLow, __builtin_fmaf(g, kHigh, -n));
+    const float m = g * __builtin_amdgcn_exp2f(f) * __builtin_amdgcn_frexp_mantf(up);
+    return gate == -__builtin_inff() ? __builtin_nanf("") : __builtin_ldexpf(m, (int)n + __builtin_amdgcn_frexp_expf(up));
 }
 
 template <typename T, int FORMAT>
@@ -182,9 +195,15 @@ __global__ __launch_bounds__(kThreads) void mx_silu_mul_kernel(const typename T:
         if (at >= count) break;
         float a[8], b[8];
         g[i].floats(a), u[i].floats(b);
+        float v[8], least = a[0];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) a[e] = silu_mul(a[e], b[e]);
-        quantize8<FORMAT>(a, codes, scales, at);
+        for (int e = 0; e < 8; ++e) v[e] = silu_mul(a[e], b[e]), least = fminf(least, a[e]);
+        if (least < kFar) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+                if (a[e] < kFar) v[e] = silu_mul_far(a[e], b[e]);
+        }
+        quantize8<FORMAT>(v, codes, scales, at);
     }
 }
 

@@ -666,3 +666,39 @@ def test_row_tiles_across_xcds(rows, k, n, fmt):
     codes, scales = nq.mx_quantize(_random(rows, rows, k), fmt)
     bias = _random(k, n, spread=False)
     _check_product(nq.mx_linear_quantized(codes, scales, w, ws, bias), (codes, scales), (w, ws), bias, torch.bfloat16)
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("dt", DT)
+def test_silu_of_gates_far_below_zero(dt, fmt):
+    """Sigmoids from 2^-58 to far past fp32's smallest value: what they give with `up` is as exact as anywhere, whole blocks of such
+    gates and single ones among others.  In fp32: the exponential to four half steps, three products and a power of two, which
+    rounds where the result is subnormal, by half of the smallest one."""
+    t = DT[dt]
+    gate = torch.cat([torch.linspace(-60, -40, 512), torch.linspace(-79, -81, 256), torch.linspace(-86, -90, 1024),
+                      torch.linspace(-110, -88, 512), torch.linspace(-300, -100, 768)]).to(t).cuda()
+    ups = (1.0, -3e-5, 6e4) if dt == "f16" else (1.0, 2.0 ** 40, -2.0 ** 100, 3e38, -2.0 ** -60, 2.0 ** -130)
+    for up in ups:
+        g = gate.unsqueeze(1).expand(-1, 32).contiguous()
+        u = torch.full_like(g, up)
+        u[:, 1::2] = -up
+        want = g.cpu().double() * torch.sigmoid(g.cpu().double()) * u.cpu().double()
+        packed = nq.mx_silu_mul(g, u, fmt)
+        _check_rounded(packed, want, fmt, 12 * U, 2.0 ** -150)
+        if abs(up) > 2.0 ** 60:
+            assert (mx.values(*packed)[gate.cpu() > -100] != 0).all()
+        # one far gate in a block whose other values are 0
+        lone = torch.zeros_like(g)
+        at = torch.arange(len(gate), device="cuda") % 32
+        lone[torch.arange(len(gate), device="cuda"), at] = gate
+        want = lone.cpu().double() * torch.sigmoid(lone.cpu().double()) * u.cpu().double()
+        _check_rounded(nq.mx_silu_mul(lone, u, fmt), want, fmt, 12 * U, 2.0 ** -150)
+
+
+def test_silu_of_infinities_with_any_up():
+    """-inf and NaN make their block NaN, as does an infinite `up`; finite gates below fp32's exponential do not."""
+    for g, u, nan in ((float("-inf"), 2.0, True), (float("nan"), 2.0, True), (-3e38, 2.0, False), (-3e38, 3e38, False), (-500.0, float("inf"), True),
+                      (-90.0, float("nan"), True), (-3e38, 0.0, False), (float("-inf"), 0.0, True)):
+        gate, up = torch.full((1, 32), g, device="cuda"), torch.full((1, 32), u, device="cuda")
+        v = mx.values(*nq.mx_silu_mul(gate, up, "mxfp8"))
+        assert bool(torch.isnan(v).all()) == nan and (nan or bool((v == 0).all()))
