@@ -17,7 +17,7 @@
  *
  * Conventions: device pointers on the current HIP device, 16-byte aligned except scales and biases (any address of their
  * type).  `dtype` is the type of the unquantised tensors of a call.  Strides are in elements, rows start on 16-byte
- * boundaries.  A call has fewer than 2^36 values of x and k <= 2^30, a product rows <= 2^20 and n <= 2^29; 0 rows (and n = 0)
+ * boundaries.  A call has at most 2^36 - 2^12 values of x and k <= 2^30, a product rows <= 2^20 and n <= 2^29; 0 rows (and n = 0)
  * are nothing to do, and no pointer is looked at then.  `stream` is a hipStream_t as void*; calls are asynchronous on it, allocate nothing and can be captured.
  * Inputs are not written.  Results do not depend on what else runs, and equal calls give equal bits.  The return value is 0
  * or an NQX_ERR code, nqx_last_error() holds the message of the calling thread's last failure.  The reference has no
@@ -73,8 +73,8 @@ int nqx_add_rmsnorm(const void* x, int64_t x_stride, const void* delta, int64_t 
                     void* total, uint8_t* codes, uint8_t* scales, int64_t rows, int64_t k, float eps, int dtype, int format,
                     void* stream);
 
-/* codes, scales of SiLU(gate) * up = gate / (1 + exp(-gate)) * up, computed in fp32, as gate * exp(gate) * up where gate is far below
- * zero: a result is right wherever it is one of fp32's, also of gates whose exp(-gate) is past fp32.  A gate of -inf gives NaN.
+/* codes, scales of SiLU(gate) * up = gate / (1 + exp(-gate)) * up, computed in fp32; where gate is far below zero as
+ * gate * exp(gate) * up, so that results are kept whose exp(-gate) is past fp32.  A gate of -inf gives NaN.
  * gate and up [rows, k], rows gate_stride and up_stride apart (2 k for the halves of one tensor). */
 int nqx_silu_mul(const void* gate, int64_t gate_stride, const void* up, int64_t up_stride, uint8_t* codes, uint8_t* scales,
                  int64_t rows, int64_t k, int dtype, int format, void* stream);

@@ -29,8 +29,9 @@ int check_types(const char* fn, int64_t rows, int64_t k, int dtype, int format) 
     if (rows < 0 || k <= 0 || k % kBlock != 0)
         return refuse(NQX_ERR_ARG, "%s: rows must not be negative and k a positive multiple of %d (rows=%lld k=%lld)", fn, kBlock,
                       (long long)rows, (long long)k);
-    // 2^36 values: a launch has fewer than 2^32 threads along x, and a thread has 16 values
-    if (k > ((int64_t)1 << 30) || rows > ((int64_t)1 << 31) || rows * (k / kBlock) >= ((int64_t)1 << 31))
+    // 2^36 values less one workgroup's: a launch has fewer than 2^32 threads along x in whole workgroups of 256, and a thread has 16
+    // values at least, half a block
+    if (k > ((int64_t)1 << 30) || rows > ((int64_t)1 << 31) || rows * (k / kBlock) > ((int64_t)1 << 31) - 128)
         return refuse(NQX_ERR_UNSUPPORTED, "%s: problem too large (rows=%lld k=%lld)", fn, (long long)rows, (long long)k);
     return NQX_OK;
 }

@@ -195,3 +195,11 @@ def test_sizes_past_a_launch_are_refused():
     assert L.nqx_add_rmsnorm(at, 32, None, 0, at, None, at, at, 1 << 24, 32, 1e-6, 1, 0, None) == 2 and b"2^24" in L.nqx_last_error()
     assert L.nqx_linear_workspace_bytes(1, (1 << 29) + 1, 32, 1, 0, 0) == 0
     assert L.nqx_linear(at, 32, at, at, None, at, 1, (1 << 29) + 1, 32, 1, 0, None, 0, None) == 2
+
+
+def test_largest_sizes_of_a_launch():
+    """The last sizes below 2^36 values, whose last workgroup would be past 2^32 threads, are refused by name, not by the launch."""
+    L, at = _lib.mx_lib(), 4096
+    for rows, k in (((1 << 31) - 1, 32), ((1 << 31) - 127, 32), (((1 << 31) - 1) // 3, 96)):
+        assert L.nqx_silu_mul(at, k, at, k, at, at, rows, k, 1, 0, None) == 2 and b"too large" in L.nqx_last_error()
+        assert L.nqx_quantize(at, k, at, at, rows, k, 1, 0, None) == 2 and L.nqx_dequantize(at, at, at, rows, k, 1, 0, None) == 2
