@@ -96,11 +96,15 @@ int64_t check_weight(const at::Tensor& weight, const at::Tensor& weight_scales, 
     TORCH_CHECK(w.k == k, "weight has ", w.k, " input features, and x ", k);
     return weight.size(0);
 }
-at::Tensor dense_bias(const OptTensor& bias, const at::Tensor& x, int64_t n, at::ScalarType dtype) {
-    if (!bias.has_value() || !bias->defined()) return {};
+// Whether there is a bias, which fits then.
+bool check_bias(const OptTensor& bias, const at::Tensor& x, int64_t n) {
+    if (!bias.has_value() || !bias->defined()) return false;
     TORCH_CHECK(bias->dim() == 1 && bias->size(0) == n, "bias must have ", n, " elements, got ", bias->sizes());
     check_device(x, {&*bias});
-    return bias->to(dtype).contiguous();
+    return true;
+}
+at::Tensor dense_bias(const OptTensor& bias, const at::Tensor& x, int64_t n, at::ScalarType dtype) {
+    return check_bias(bias, x, n) ? bias->to(dtype).contiguous() : at::Tensor();
 }
 
 Two mx_quantize(const at::Tensor& x, c10::string_view format) {
@@ -135,7 +139,9 @@ at::Tensor mx_dequantize(const at::Tensor& codes, const at::Tensor& scales, at::
 }
 at::Tensor mx_dequantize_meta(const at::Tensor& codes, const at::Tensor& scales, at::ScalarType dtype) {
     dtype_id(dtype);
-    return empty_beside(codes, with_last(codes, check_packed(codes, scales, "mx_dequantize").k), dtype);
+    const Packed p = check_packed(codes, scales, "mx_dequantize");
+    check_device(codes, {&scales});
+    return empty_beside(codes, with_last(codes, p.k), dtype);
 }
 
 at::Tensor mx_linear(const at::Tensor& x, const at::Tensor& weight, const at::Tensor& weight_scales, const OptTensor& bias,
@@ -156,11 +162,14 @@ at::Tensor mx_linear(const at::Tensor& x, const at::Tensor& weight, const at::Te
                  "nqx_linear");
     return y;
 }
-at::Tensor mx_linear_meta(const at::Tensor& x, const at::Tensor& weight, const at::Tensor& weight_scales, const OptTensor&,
+at::Tensor mx_linear_meta(const at::Tensor& x, const at::Tensor& weight, const at::Tensor& weight_scales, const OptTensor& bias,
                           c10::string_view activations) {
     format_id(activations);
     dtype_id(x.scalar_type());
-    return empty_beside(x, with_last(x, check_weight(weight, weight_scales, last_size(x, "x"))), x.scalar_type());
+    const int64_t n = check_weight(weight, weight_scales, last_size(x, "x"));
+    check_device(x, {&weight, &weight_scales});
+    check_bias(bias, x, n);
+    return empty_beside(x, with_last(x, n), x.scalar_type());
 }
 
 at::Tensor mx_linear_quantized(const at::Tensor& codes, const at::Tensor& scales, const at::Tensor& weight, const at::Tensor& weight_scales,
@@ -184,9 +193,12 @@ at::Tensor mx_linear_quantized(const at::Tensor& codes, const at::Tensor& scales
     return y;
 }
 at::Tensor mx_linear_quantized_meta(const at::Tensor& codes, const at::Tensor& scales, const at::Tensor& weight,
-                                    const at::Tensor& weight_scales, const OptTensor&, at::ScalarType dtype) {
+                                    const at::Tensor& weight_scales, const OptTensor& bias, at::ScalarType dtype) {
     dtype_id(dtype);
-    return empty_beside(codes, with_last(codes, check_weight(weight, weight_scales, check_packed(codes, scales, "x").k)), dtype);
+    const int64_t n = check_weight(weight, weight_scales, check_packed(codes, scales, "x").k);
+    check_device(codes, {&scales, &weight, &weight_scales});
+    check_bias(bias, codes, n);
+    return empty_beside(codes, with_last(codes, n), dtype);
 }
 
 void check_norm(const at::Tensor& x, const at::Tensor& weight) {
@@ -226,6 +238,7 @@ Three mx_add_rmsnorm_meta(const at::Tensor& x, const at::Tensor& delta, const at
     dtype_id(x.scalar_type());
     check_norm(x, weight);
     check_alike(x, delta, "x and delta");
+    check_device(x, {&delta, &weight});
     Two out = packed_like(x, format_id(format));
     return {std::get<0>(out), std::get<1>(out), empty_beside(x, x.sizes(), x.scalar_type())};
 }
@@ -240,6 +253,7 @@ Two mx_rmsnorm(const at::Tensor& x, const at::Tensor& weight, double eps, c10::s
 Two mx_rmsnorm_meta(const at::Tensor& x, const at::Tensor& weight, double, c10::string_view format) {
     dtype_id(x.scalar_type());
     check_norm(x, weight);
+    check_device(x, {&weight});
     return packed_like(x, format_id(format));
 }
 
@@ -261,6 +275,7 @@ Two mx_silu_mul_meta(const at::Tensor& gate, const at::Tensor& up, c10::string_v
     dtype_id(gate.scalar_type());
     last_size(gate, "gate");
     check_alike(gate, up, "gate and up");
+    check_device(gate, {&up});
     return packed_like(gate, format_id(format));
 }
 

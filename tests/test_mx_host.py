@@ -203,3 +203,22 @@ def test_largest_sizes_of_a_launch():
     for rows, k in (((1 << 31) - 1, 32), ((1 << 31) - 127, 32), (((1 << 31) - 1) // 3, 96)):
         assert L.nqx_silu_mul(at, k, at, k, at, at, rows, k, 1, 0, None) == 2 and b"too large" in L.nqx_last_error()
         assert L.nqx_quantize(at, k, at, at, rows, k, 1, 0, None) == 2 and L.nqx_dequantize(at, at, at, rows, k, 1, 0, None) == 2
+
+
+def test_meta_kernels_check_what_device_kernels_check():
+    """A bias of another size or rank, and tensors of two devices, pass neither tracing nor the device."""
+    ops = _lib.mx_ops()
+    w, ws, x = _meta(7, 48, dtype=torch.uint8), _meta(7, 3, dtype=torch.uint8), _meta(4, 96)
+    c8, s = _meta(4, 96, dtype=torch.uint8), _meta(4, 3, dtype=torch.uint8)
+    for good in (None, _meta(7), _meta(7, dtype=torch.float32), _meta(7, dtype=torch.float16)):
+        assert ops.mx_linear(x, w, ws, good, "mxfp8").shape == ops.mx_linear_quantized(c8, s, w, ws, good, torch.float16).shape == (4, 7)
+    for bad in (_meta(8), _meta(1), _meta(7, 1), _meta(0), torch.zeros(7, dtype=torch.bfloat16)):
+        for call in (lambda: ops.mx_linear(x, w, ws, bad, "mxfp8"), lambda: ops.mx_linear_quantized(c8, s, w, ws, bad, torch.float16)):
+            with pytest.raises(RuntimeError):
+                call()
+    cpu, cpu8 = torch.zeros(4, 96, dtype=torch.bfloat16), torch.zeros(4, 3, dtype=torch.uint8)
+    for call in (lambda: ops.mx_linear(x, torch.zeros(7, 48, dtype=torch.uint8), ws, None, "mxfp8"), lambda: ops.mx_dequantize(c8, cpu8, torch.float16),
+                 lambda: ops.mx_linear_quantized(c8, cpu8, w, ws, None, torch.float16), lambda: ops.mx_silu_mul(x, cpu, "mxfp8"),
+                 lambda: ops.mx_add_rmsnorm(x, cpu, _meta(96), 1e-6, "mxfp8"), lambda: ops.mx_rmsnorm(x, cpu[0], 1e-6, "mxfp8")):
+        with pytest.raises(RuntimeError):
+            call()
