@@ -55,7 +55,7 @@ def mx_dequantize(codes: torch.Tensor, scales: torch.Tensor, dtype: torch.dtype 
 def mx_linear(x: torch.Tensor, weight: torch.Tensor, weight_scales: torch.Tensor, bias: Optional[torch.Tensor] = None,
               activations: str = "mxfp8") -> torch.Tensor:
     """x [..., k] quantised to `activations`, times weight^T, plus bias: [..., n] in x's dtype.  Sums in fp32, one rounding
-    behind the bias."""
+    behind the bias.  A bias of another dtype than x is rounded to x's first, by a launch of its own."""
     if not x.is_cuda:
         raise _elsewhere(x)
     return _ops.mx_linear(x, weight, weight_scales, bias, activations)
@@ -63,7 +63,8 @@ def mx_linear(x: torch.Tensor, weight: torch.Tensor, weight_scales: torch.Tensor
 
 def mx_linear_quantized(codes: torch.Tensor, scales: torch.Tensor, weight: torch.Tensor, weight_scales: torch.Tensor,
                         bias: Optional[torch.Tensor] = None, dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
-    """The same product for activations that are quantised already (by mx_quantize, mx_add_rmsnorm or mx_silu_mul)."""
+    """The same product for activations that are quantised already (by mx_quantize, mx_add_rmsnorm or mx_silu_mul); `dtype` takes
+    the place of x's."""
     if not codes.is_cuda:
         raise _elsewhere(codes)
     return _ops.mx_linear_quantized(codes, scales, weight, weight_scales, bias, dtype)
@@ -107,13 +108,14 @@ class MXLinear(nn.Module):
     @classmethod
     def from_linear(cls, linear: nn.Linear, activations: str = "mxfp8",
                     output_dtype: Optional[torch.dtype] = None) -> "MXLinear":
-        """Quantises the weight of a linear that lies on a HIP device."""
+        """Quantises the weight of a linear that lies on a HIP device.  `output_dtype` is that of its bias too; without one results
+        of (codes, scales) are of the weight's dtype, or bfloat16 for a float32 weight, and the bias is held as the linear has it."""
         w = linear.weight.detach()
         made = cls(linear.in_features, linear.out_features, linear.bias is not None, activations, "meta",
                    output_dtype or (w.dtype if w.dtype != torch.float32 else torch.bfloat16))
         made.weight, made.weight_scales = mx_quantize(w, "mxfp4")
         if linear.bias is not None:
-            made.bias = linear.bias.detach().to(made.output_dtype, copy=True)
+            made.bias = linear.bias.detach().to(output_dtype or linear.bias.dtype, copy=True)
         return made
 
     def forward(self, x) -> torch.Tensor:

@@ -702,3 +702,25 @@ def test_silu_of_infinities_with_any_up():
         gate, up = torch.full((1, 32), g, device="cuda"), torch.full((1, 32), u, device="cuda")
         v = mx.values(*nq.mx_silu_mul(gate, up, "mxfp8"))
         assert bool(torch.isnan(v).all()) == nan and (nan or bool((v == 0).all()))
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+def test_bias_of_a_float32_linear(fmt):
+    """It is held as it is, so that float32 x gets all of it; a result of 16 bits gets it rounded to that type."""
+    torch.manual_seed(3)
+    lin = torch.nn.Linear(160, 48, device="cuda")
+    lin.bias.data.copy_(_random(5, 48, dtype=torch.float32, spread=False))
+    m = nq.MXLinear.from_linear(lin, fmt)
+    assert torch.equal(m.bias, lin.bias) and m.bias.data_ptr() != lin.bias.data_ptr() and m.output_dtype == torch.bfloat16
+    for rows in (1, 40, 300):
+        x = _random(rows, rows, 160, dtype=torch.float32)
+        packed = nq.mx_quantize(x, fmt)
+        y = m(x)
+        _check_product(y, packed, (m.weight, m.weight_scales), lin.bias.detach(), torch.float32)
+        y = m(packed)
+        _check_product(y, packed, (m.weight, m.weight_scales), lin.bias.detach().bfloat16(), torch.bfloat16)
+    told = nq.MXLinear.from_linear(lin, fmt, torch.float16)
+    assert told.bias.dtype == told.output_dtype == told(packed).dtype == torch.float16 and torch.equal(told.bias, lin.bias.half())
+    same = nq.MXLinear(160, 48, True, fmt, "cuda").float()       # uint8 buffers stay
+    same.load_state_dict(m.state_dict())
+    assert torch.equal(same(x), m(x)) and torch.equal(same(packed), m(packed))
