@@ -724,3 +724,32 @@ def test_bias_of_a_float32_linear(fmt):
     same = nq.MXLinear(160, 48, True, fmt, "cuda").float()       # uint8 buffers stay
     same.load_state_dict(m.state_dict())
     assert torch.equal(same(x), m(x)) and torch.equal(same(packed), m(packed))
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("dt", ["bf16", "f32"])
+def test_norm_of_squares_past_fp32(dt, fmt):
+    """Rows of the type's largest values, and of one such value among others: their mean is infinity, and they become zeros; rows
+    beside them are as without."""
+    t, k = DT[dt], 544
+    weight, x = _random(1, k, dtype=t, spread=False), _random(2, 5, k, dtype=t)
+    want = nq.mx_add_rmsnorm(x, None, weight, 1e-6, fmt)
+    bad = x.clone()
+    bad[1] = torch.finfo(t).max
+    bad[1, ::2] = -torch.finfo(t).max
+    bad[3, 500] = 2.0 ** 64                                   # its square alone is past fp32
+    for got in (nq.mx_add_rmsnorm(bad, None, weight, 1e-6, fmt), nq.mx_add_rmsnorm(bad, torch.zeros_like(bad), weight, 1e-6, fmt)):
+        v = mx.values(*got[:2])
+        assert (v[1] == 0).all() and (v[3] == 0).all() and torch.equal(got[2], bad)
+        assert all(torch.equal(got[i][::2], want[i][::2]) for i in (0, 1))
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+def test_norm_just_below(fmt):
+    """Squares whose sum is just in fp32, and those that vanish beside eps."""
+    k = 1024
+    weight = torch.ones(k, device="cuda")
+    x = torch.stack([torch.full((k,), v, device="cuda") for v in (2.0 ** 58, -2.0 ** 58, 2.0 ** -40, 2.0 ** -80)])
+    codes, scales, _ = nq.mx_add_rmsnorm(x, None, weight, 1e-6, fmt)
+    s = x.cpu().double()
+    _check_rounded((codes, scales), s / torch.sqrt((s * s).mean(-1, keepdim=True) + 1e-6), fmt, 16 * U)
