@@ -1,8 +1,8 @@
 // Row kernels of the microscaled formats: quantise, dequantise, residual addition + RMSNorm, SiLU(gate) * up.  All are
 // bound by memory: a lane takes eight consecutive values in one or two 16-byte loads, several eights at once, the four lanes of
-// a block agree on the largest magnitude by two DPP moves, and codes leave in 4- or 8-byte stores, whole lines a wave.  In bf16,
-// 25600 x 5120: quantise to e2m1 67 us (5.0 TB/s; 88 to e4m3, 4.5), dequantise 53 and 58 (6.3 and 6.8 with the codes still in
-// the last cache); 8192 x 5120: sum, norm and e4m3 63 us (4.7 TB/s).  A large copy reaches 5.2.
+// a block agree on the largest magnitude by two DPP moves, and codes leave in 4- or 8-byte stores, whole lines a wave.  In bf16, on
+// tensors that are in no cache, 25600 x 5120: quantise to e2m1 59 us, to e4m3 70 (5.6 and 5.7 TB/s), dequantise 59 and 68 (5.6 and
+// 5.8); 8192 x 5120: sum, norm and e4m3 54 us (5.4 TB/s); 8192 x 12288: SiLU to e2m1 84 us (5.5 TB/s).  A large copy reaches 5.1.
 #include "mx_common.hpp"
 
 namespace nqx {
@@ -154,7 +154,7 @@ __global__ __launch_bounds__(kThreads) void mx_add_rmsnorm_kernel(const typename
 // gate / (1 + exp(-gate)) * up.  exp(-g) is 2^t 2^r, t = -g log2(e) rounded and r what that and the constant lost: without r the
 // relative error grows with |g|.  (2^r as a factor of its own near 1: where 2^t is infinite a sum could be inf - inf.)  The
 // reciprocal is off by a step of fp32 at most, a division would be by half of one and takes ten times as long (8192 x 12288 bf16
-// to e2m1 is 102 us, 4.5 TB/s, and was 116 with expf and a division).  Above 100 the exponential does not change 1.  For gates
+// to e2m1 is 84 us, and 97 with expf and a division; to e4m3 91 and 103).  Above 100 the exponential does not change 1.  For gates
 // below kFar the result is silu_mul_far's: the hardware reciprocal has no subnormal results, so from -87.3 on it would be 0, which a
 // large `up` would make of values that are not small.
 constexpr float kHigh = 1.44269502f, kLow = 1.92596303e-8f;       // log2(e) in two parts

@@ -4,8 +4,9 @@
 // one barrier a chunk.  (x comes from a cache, but its requests return behind the weight's: asked for one chunk ahead a chunk of 64
 // rows took 2.5 us.  Three chunks ahead gain nothing: 41 rows by 25600 x 5120 in 4 bits 21.6 us and 21.4.)  Where the weight has too
 // few rows for the chip, k is split over workgroups, whose sums go to memory in fp32 and are added, in the order of the splits, by a
-// second kernel.  Up to 64 rows are bound by the weight's bytes (16 by 5120 x 25600 12.3 us, 5.7 TB/s), more by what a CU gets from
-// L2 and LDS (333 by 2816 x 9728 in 8 bits 1.1 us a chunk, of which the matrix instructions need half).
+// second kernel.  Up to 64 rows are bound by the weight's bytes (16 by 5120 x 25600 12.5 us, 5.6 TB/s, with the weight in the last cache,
+// and 16.6 from memory).  More rows: a wave reads a chunk's fragments behind its barrier and then multiplies them, and with all waves in
+// step the two hardly overlap (333 by 2816 x 9728 in 8 bits 1.1 us a chunk: 0.5 us of matrix instructions, and 0.7 without them).
 //
 // With RAW x comes as it is and every workgroup quantises its run of it into LDS first, while its first chunks are on their way:
 // one launch for a linear of few rows.
@@ -26,8 +27,8 @@ int sixteens(int64_t rows) { return rows <= 16 ? 1 : rows <= 32 ? 2 : rows <= 64
 // Splits of k: at most as many as fill the chip with workgroups that are resident at once, of four chunks each at least, and of those
 // the number that costs least: the longest split's chunks or, if that is more, the weight's way from memory, and where there is more
 // than one a launch and the sums' way to memory and back.  Nanoseconds of a chunk and of a launch and 5.2 TB/s as measured; 128 rows by 2560 x 9728 in 8 bits 18.0 us with two splits and 15.2
-// with one, 64 rows in 4 bits 11.7 and 9.5; 16 rows by 5120 x 25600 17.9
-// and 15.2.  (Workgroups of 256 weight rows would share x among more of them: 41 rows by
+// with one, 64 rows in 4 bits 11.7 and 9.5; 16 rows by 5120 x 25600, from
+// memory, 20.2 and 16.7.  (Workgroups of 256 weight rows would share x among more of them: 41 rows by
 // 25600 x 5120 26.5 us and 24.5 with 128, 64 rows by 4096 x 12288 17.6 and 14.3.)
 int splits_of(int64_t rows, int64_t n, int64_t k, int format) {
     const int mt = sixteens(rows);
@@ -381,7 +382,7 @@ __global__ __launch_bounds__(256 * fours(MT)) void mx_stream_kernel(const void* 
 template <typename T>
 __global__ __launch_bounds__(256) void mx_add_splits_kernel(const float* __restrict__ sums, const typename T::elem* __restrict__ bias,
                                                             typename T::elem* __restrict__ y, int rows, int N, int pitch, int splits) {
-    // fewer than 160 tiles of 128 x 128 sums: 32 bits
+    // a split product has at most 256 tiles of 16 x 128 sums or 128 of up to 128 x 128: 32 bits
     const uint32_t at = (blockIdx.x * 256 + threadIdx.x) * 4, m = at / (uint32_t)pitch, n = at - m * pitch;
     if (m >= (uint32_t)rows || n >= (uint32_t)N) return;
     float b[4] = {};

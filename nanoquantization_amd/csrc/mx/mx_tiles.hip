@@ -14,7 +14,7 @@ namespace nqx {
 namespace {
 
 // What the matrix instruction takes at once.  e2m1 on both sides runs on 32 x 32 x 64 (a loop of nothing else reaches 6.4
-// PFLOP/s, one of 16 x 16 x 128 5.1); e4m3 with e2m1 on 16 x 16 x 128 (4.2, and 3.9 on 32 x 32 x 64).
+// PFLOP/s, one of 16 x 16 x 128 5.1); e4m3 with e2m1 on 16 x 16 x 128 (4.0 to 4.2, by the GPU, and 3.5 to 3.9 on 32 x 32 x 64).
 template <int FORMAT>
 struct Shape {
     static constexpr int kRows = 16;
@@ -170,7 +170,8 @@ __global__ __launch_bounds__(256, (S == 256 ? 1 : 2)) void mx_tiles_kernel(
             for (int q = 0; q < G::kLoads; ++q) load_x(q, 1);
         }
     }
-    // what goes out behind the barrier of a chunk that does not exist
+    // What goes out behind the barrier of a chunk that does not exist.  (In e2m1, and in e4m3 tiles of 256, a part of it goes out
+    // in the first chunk's steps once more, to the same place, which nobody reads before the barrier behind both.)
     if (kFour) {
 #pragma unroll
         for (int q = 0; q < G::kLoads; ++q) load_w(q, 1), load_x(q, 1);
